@@ -1,0 +1,121 @@
+"""Rotary position embedding with several position axes (time, height, width for images and video).
+
+No counterpart in the reference, whose rotary kernels take one row of cos / sin per token
+(python/dlBLAS/dlblas/kernels/apply_rotary_pos_emb.py:98)."""
+from __future__ import annotations
+
+import ctypes
+from functools import lru_cache
+from typing import Sequence
+
+import torch
+from torch import Tensor
+
+from .. import _lib
+
+
+@lru_cache(maxsize=64)
+def _axis_of_freq(sections: tuple, interleaved: bool):
+    """Axis of every frequency as a host byte array."""
+    if interleaved:
+        order = sorted((i, a) for a, n in enumerate(sections) for i in range(n))
+        axes = [a for _, a in order]
+    else:
+        axes = [a for a, n in enumerate(sections) for _ in range(n)]
+    return (ctypes.c_uint8 * max(len(axes), 1))(*axes)
+
+
+def _launch(q, k, q_out, k_out, positions, inv_freq, axes, inverse):
+    tokens, hq, dim = q.shape
+    qs, ks, qos, kos = q.stride(), k.stride(), q_out.stride(), k_out.stride()
+    lib = _lib.load()
+    dev = q.device
+    with _lib.on_device(dev):
+        rc = lib.dlb_multi_axis_rotary(
+            q.data_ptr(), k.data_ptr(), q_out.data_ptr(), k_out.data_ptr(), positions.data_ptr(),
+            int(positions.dtype == torch.int64), positions.stride(0), inv_freq.data_ptr(), axes, positions.size(0),
+            tokens, hq, k.size(1), dim, 2 * inv_freq.numel(), qs[0], qs[1], ks[0], ks[1], qos[0], qos[1], kos[0],
+            kos[1], int(inverse), _lib.dtype_code(q), _lib.stream_ptr(dev))
+    _lib.check(rc, "apply_multi_axis_rotary")
+
+
+def _dense(t):
+    return t if t.stride(-1) == 1 or t.size(-1) == 1 else t.contiguous()
+
+
+class _MultiAxisRotary(torch.autograd.Function):
+    """The gradient of a rotation is the rotation back, so the backward pass is this function with the other sign (and
+    can be differentiated again)."""
+
+    @staticmethod
+    def forward(ctx, q, k, positions, inv_freq, axes, inverse):
+        ctx.save_for_backward(positions, inv_freq)
+        ctx.axes, ctx.inverse = axes, inverse
+        ctx.set_materialize_grads(False)
+        q_out, k_out = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k))
+        _launch(_dense(q), _dense(k), q_out, k_out, positions, inv_freq, axes, inverse)
+        return q_out, k_out
+
+    @staticmethod
+    def backward(ctx, grad_q, grad_k):
+        if grad_q is None and grad_k is None:
+            return (None,) * 6
+        positions, inv_freq = ctx.saved_tensors
+        # an output that nothing was made of has no gradient: its heads are left out of the launch
+        some = grad_k if grad_q is None else grad_q
+        none = some.new_empty((some.size(0), 0, some.size(2)))
+        dq, dk = _MultiAxisRotary.apply(none if grad_q is None else grad_q, none if grad_k is None else grad_k,
+                                        positions, inv_freq, ctx.axes, not ctx.inverse)
+        return None if grad_q is None else dq, None if grad_k is None else dk, None, None, None, None
+
+
+def apply_multi_axis_rotary(
+    q: Tensor,
+    k: Tensor,
+    positions: Tensor,
+    inv_freq: Tensor,
+    sections: Sequence[int],
+    interleaved: bool = False,
+    q_embed: Tensor = None,
+    k_embed: Tensor = None,
+):
+    """Rotate-half rotary embedding of query and key ([tokens, heads, dim]) at positions with several axes.
+
+    `positions` [axes, tokens] (int32 or int64, 1 to 8 axes) holds each token's place on every axis, `inv_freq` (fp32,
+    up to dim / 2 and 256 of them) the angle per step of each frequency; the first `2 * len(inv_freq)` columns are
+    rotated (column f with column f + len(inv_freq)), the others pass through.  `sections[a]` frequencies follow axis
+    a: the first sections[0] frequencies the first axis and so on, or, with `interleaved`, one frequency to each axis
+    in turn, an axis dropping out once it has its number.  Angles are formed in 64 bits and the rotation in 32, with
+    one rounding to the tensors' type (fp16, bf16, fp32): no cos / sin tables, and positions far out stay exact.
+
+    Differentiable in q and k where one of them requires a gradient; `q_embed` / `k_embed` (which may be the inputs)
+    are for calls without one.  Returns (q_embed, k_embed).
+    """
+    dev = _lib.require_cuda(q, k, positions, inv_freq, q_embed, k_embed)
+    assert q.dim() == 3 and k.dim() == 3 and k.size(0) == q.size(0) and k.size(2) == q.size(2), \
+        "q and k are [tokens, heads, dim] with the same tokens and dim"
+    assert k.dtype == q.dtype, "q and k must have one dtype"
+    assert positions.dim() == 2 and positions.size(1) == q.size(0), "positions are [axes, tokens]"
+    assert positions.dtype in (torch.int32, torch.int64), "positions must be int32 or int64"
+    assert inv_freq.dim() == 1 and inv_freq.dtype == torch.float32, "inv_freq is a vector of fp32"
+    assert not inv_freq.requires_grad, "there is no gradient for inv_freq"
+    sections = tuple(int(n) for n in sections)
+    assert len(sections) == positions.size(0) and min(sections) >= 0 and sum(sections) == inv_freq.numel(), \
+        "sections: one count per axis, together as many as frequencies"
+    axes = _axis_of_freq(sections, bool(interleaved))
+    if positions.stride(1) != 1:
+        positions = positions.contiguous()
+    inv_freq = inv_freq.contiguous()
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad):
+        assert q_embed is None and k_embed is None, "outputs cannot be given where a gradient is wanted"
+        return _MultiAxisRotary.apply(q, k, positions, inv_freq, axes, False)
+    q, k = _dense(q), _dense(k)
+    if q_embed is None:
+        q_embed = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    if k_embed is None:
+        k_embed = torch.empty(k.shape, dtype=k.dtype, device=dev)
+    for out, x in ((q_embed, q), (k_embed, k)):
+        assert out.shape == x.shape and out.dtype == x.dtype and (out.stride(-1) == 1 or out.size(-1) == 1), \
+            "q_embed / k_embed must have their input's shape and dtype, the last dimension contiguous"
+    _launch(q, k, q_embed, k_embed, positions, inv_freq, axes, False)
+    return q_embed, k_embed

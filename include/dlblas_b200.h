@@ -305,6 +305,19 @@ int dlb_apply_rotary(const void* q, const void* k, const void* cos, const void* 
                      int64_t k_stride_t, int64_t k_stride_h, int64_t qo_stride_t, int64_t qo_stride_h,
                      int64_t ko_stride_t, int64_t ko_stride_h, int dtype, void* stream);
 
+/* Rotary position embedding with several position axes: frequency f (of rot_dim / 2, at most 256) turns the columns
+ * (f, f + rot_dim / 2) of every head by positions[axis_of_freq[f]][token] * inv_freq[f], columns from rot_dim on pass
+ * through; inverse != 0 turns back (the gradient).  positions int32 or int64 [axes, tokens] with position_stride
+ * between axes (1 to 8 of them), inv_freq fp32 [rot_dim / 2], axis_of_freq a HOST array of rot_dim / 2 bytes that is
+ * read during the call.  Angles in 64 bits, the rotation in 32, one rounding.  Outputs may be the inputs (same pointer
+ * and strides); hq or hk may be 0.  No counterpart in the reference. */
+int dlb_multi_axis_rotary(const void* q, const void* k, void* q_out, void* k_out, const void* positions,
+                          int positions_are_int64, int64_t position_stride, const float* inv_freq,
+                          const uint8_t* axis_of_freq, int axes, int64_t tokens, int hq, int hk, int dim, int rot_dim,
+                          int64_t q_stride_t, int64_t q_stride_h, int64_t k_stride_t, int64_t k_stride_h,
+                          int64_t qo_stride_t, int64_t qo_stride_h, int64_t ko_stride_t, int64_t ko_stride_h,
+                          int inverse, int dtype, void* stream);
+
 /* Scatter the new tokens' key/value states into the paged caches [pages, page_size, heads, d]:
  * token i of sequence b lands in slot (history + i) % page_size of page
  * block_offsets[b, (history + i) / page_size], history = kv_seq_length[b] - q_seq_length[b].
