@@ -16,7 +16,7 @@ LIB_PATH = os.path.join(_PKG_DIR, "libdlblas_b200.so")
 
 DTYPE_F16, DTYPE_BF16, DTYPE_F32 = 0, 1, 2
 SCORE_SIGMOID, SCORE_SOFTMAX = 0, 1
-DEV_BAD_ROW = 2  # code in a device status word
+DEV_BAD_ROW, DEV_BAD_PAGE = 2, 3  # codes in a device status word
 GEMM_FUSE_SILU, GEMM_WEIGHT, GEMM_SCATTER, GEMM_PEER, GEMM_SLOTS_ONLY = 1, 2, 4, 8, 16
 
 _DTYPES = {torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16, torch.float32: DTYPE_F32}
@@ -85,6 +85,11 @@ SIGNATURES = {
                                  c_void_p]),
     "dlb_multi_axis_rotary": (c_int, [c_void_p] * 5 + [c_int, c_int64, c_void_p, c_void_p, c_int, c_int64] +
                               [c_int] * 4 + [c_int64] * 8 + [c_int, c_int, c_void_p]),
+    "dlb_sink_attention": (c_int, [c_void_p] * 8 + [c_int64] * 21 + [c_int] * 4 + [c_int64] * 2 + [c_float] * 2 +
+                           [c_int, c_void_p, c_void_p]),
+    "dlb_shared_prefix_workspace_floats": (c_int64, [c_int64] * 4),
+    "dlb_shared_prefix_attention": (c_int, [c_void_p] * 10 + [c_int64] * 22 + [c_int] * 5 + [c_int64] + [c_float] * 2 +
+                                    [c_int, c_void_p, c_void_p]),
     "dlb_fill_kv_cache": (c_int, [c_void_p] * 8 + [c_int64] * 19 + [c_int] * 5 + [c_void_p, c_void_p, c_int, c_void_p]),
     "dlb_paged_decode_static": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                         c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64,
@@ -190,7 +195,7 @@ _status_words: dict[int, torch.Tensor] = {}
 
 
 def status_word(device: torch.device) -> torch.Tensor:
-    """Per-device int32[4] that a kernel writes when a bounded wait gives up or a table row does not exist."""
+    """Per-device int32[4] that a kernel writes when a bounded wait gives up or a table row or page does not exist."""
     idx = device.index if device.index is not None else torch.cuda.current_device()
     t = _status_words.get(idx)
     if t is None:
@@ -212,7 +217,7 @@ def set_wait_budget_ms(ms: int) -> None:
 
 
 def check_device_status(device=None) -> None:
-    """Synchronise and raise if any kernel recorded a timed-out wait or a bad table row since the last check."""
+    """Synchronise and raise if any kernel recorded a timed-out wait or a bad table row or page since the last check."""
     devs = list(_status_words) if device is None else [torch.device(device).index or 0]
     for idx in devs:
         t = _status_words.get(idx)
@@ -224,5 +229,8 @@ def check_device_status(device=None) -> None:
             if vals[0] == DEV_BAD_ROW:
                 raise DlblasError(f"device status on cuda:{idx}: request {vals[1]} of a decode asked for row {vals[3]} "
                                   f"of a table of {vals[2]}")
+            if vals[0] == DEV_BAD_PAGE:
+                raise DlblasError(f"device status on cuda:{idx}: row {vals[1]}, column {vals[2]} of a block table names "
+                                  f"page {vals[3]}, which the cache does not have")
             raise DlblasError(
                 f"device status on cuda:{idx}: code={vals[0]} wait_site={vals[1]} block={vals[2]} aux={vals[3]}")

@@ -48,10 +48,12 @@ struct NvtxRange {
 // Layout of the device status word array (int32[4]), written by the first kernel that has something to report:
 // [0] = code (0 = none).  A bounded wait that gave up: [1] = wait site, [2] = blockIdx.x, [3] = auxiliary value
 // (tile / iteration).  A table row that does not exist: [1] = sequence, [2] = rows of the table, [3] = the row asked for
-// (clamped to 32 bits).
+// (clamped to 32 bits).  A page that does not exist where a visible token should be: [1] = row of the table, [2] = column,
+// [3] = the page.
 #define DLB_DEV_OK 0
 #define DLB_DEV_WAIT_TIMEOUT 1
 #define DLB_DEV_BAD_ROW 2
+#define DLB_DEV_BAD_PAGE 3
 
 namespace dlb {
 

@@ -38,7 +38,7 @@
 
 #include <algorithm>
 
-#include "common.cuh"
+#include "attention.cuh"
 
 namespace dlb {
 
@@ -72,64 +72,6 @@ template <int D> struct Layout {
   static constexpr int SMEM_BYTES = OFF_CTRL + 160;   // D=128: two CTAs (plus 1 KiB system reserve each) fit one SM
 };
 }  // namespace fp
-
-static int make_tmap_tokens(CUtensorMap* out, const void* base, int64_t d, int64_t heads, int64_t tokens,
-                            int64_t stride_h, int64_t stride_t, int box_tokens) {
-  PFN_encodeTiled enc = get_encode_tiled();
-  DLB_CHECK_ARG(enc != nullptr, DLB_ERR_DRIVER, "cuTensorMapEncodeTiled is not available from the driver");
-  DLB_CHECK_ARG(((uintptr_t)base & 15) == 0, DLB_ERR_ALIGNMENT, "attention tensor base is not 16-byte aligned");
-  DLB_CHECK_ARG((stride_h * 2) % 16 == 0 && (stride_t * 2) % 16 == 0, DLB_ERR_ALIGNMENT,
-                "attention tensor strides must be multiples of 16 bytes");
-  cuuint64_t dims[3] = {(cuuint64_t)d, (cuuint64_t)heads, (cuuint64_t)tokens};
-  cuuint64_t strides[2] = {(cuuint64_t)stride_h * 2, (cuuint64_t)stride_t * 2};
-  cuuint32_t box[3] = {64, 1, (cuuint32_t)box_tokens};
-  cuuint32_t estr[3] = {1, 1, 1};
-  CUresult r = enc(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
-                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  DLB_CHECK_ARG(r == CUDA_SUCCESS, DLB_ERR_DRIVER, "cuTensorMapEncodeTiled(tokens) failed with CUresult %d", (int)r);
-  return DLB_OK;
-}
-
-__device__ __forceinline__ void tma_load_3d(void* smem_dst, const CUtensorMap* tmap, uint64_t* bar, int c0, int c1,
-                                            int c2) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
-      ::"r"(smem_u32(smem_dst)),
-      "l"(tmap), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
-      : "memory");
-}
-
-__device__ __forceinline__ float fast_exp2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
-}
-// Packed pairs of fp32 in one 64-bit register (sm_100 f32x2 arithmetic)
-__device__ __forceinline__ uint64_t pack_f2(float lo, float hi) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-  return r;
-}
-__device__ __forceinline__ void unpack_f2(uint64_t v, float& lo, float& hi) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
-}
-__device__ __forceinline__ uint64_t fma_f2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ uint64_t add_f2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
 
 struct PrefillParams {
   void* out;
@@ -167,10 +109,6 @@ struct PrefillParams {
   float softcap;                  // > 0: scores become softcap * tanh(score * sm_scale / softcap) (paged_attention.py:441-444)
   float sm_scale;
 };
-
-__device__ __forceinline__ int table_entry(const void* t, int64_t i, int is64) {
-  return is64 ? (int)reinterpret_cast<const int64_t*>(t)[i] : reinterpret_cast<const int32_t*>(t)[i];
-}
 
 // CTA index -> (sequence, row tile, q head); false if the CTA has no work.  Every warp works it out by itself.
 //   ORDER_GROUPS      (sequence, kv head) groups one after the other, inside a group the heavy (late, causal) tiles
@@ -317,7 +255,7 @@ flash_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       const int tok = (jb0 + j) * BN + u * box_slots;
       int page_slot = tok / p.page_size;
       if (page_slot >= p.max_pages) page_slot = p.max_pages - 1;   // past the table: any valid page, masked later
-      int page = table_entry(p.block_table, (int64_t)seq * p.bt_stride + page_slot, p.table_is_int64);
+      int page = load_index(p.block_table, (int64_t)seq * p.bt_stride + page_slot, p.table_is_int64);
       if (tok >= kv_len || page < 0 || page >= p.num_pages) page = 0;
       pg[u] = page;
       sl[u] = tok % p.page_size;

@@ -11,7 +11,8 @@
  *   - `status` (optional, may be NULL) is a device int32[4] the tensor-core kernels
  *     write if one of their bounded waits gives up:
  *     {code (0 = none, 1 = wait timed out), wait site, block index, tile}
- *     (dlb_paged_decode_rows has a code 2 of its own).
+ *     (dlb_paged_decode_rows has a code 2 of its own; dlb_sink_attention and dlb_shared_prefix_attention a code 3
+ *     with {row, column, page} of a table entry that names no page of the cache where a visible token should be).
  *
  * Paths below are relative to the reference project root (DeepLink-org/DLCompiler).
  */
@@ -287,6 +288,46 @@ int dlb_paged_decode_rows(const void* q, const void* k_cache, const void* v_cach
                           int64_t v_stride_page, int64_t v_stride_slot, int64_t v_stride_head, int64_t bt_stride,
                           int table_is_int64, int lens_is_int64, int64_t chunk, int64_t max_splits, int64_t window,
                           float sm_scale, float softcap, int dtype, int32_t* status, void* stream);
+
+/* Attention over a paged cache with a sliding window and sinks: the query at position p sees the keys j <= p with
+ * j >= p - window or j < sinks.  q [total_q_tokens, hq, head_dim] packed by q_start_loc / q_seq_len, out
+ * [total_q_tokens, hq, head_dim_v], caches [num_pages, page_size, hkv, d] (page_size a power of two >= 16) that already
+ * hold the new tokens, block_table [batch, max_pages], kv_seq_len [batch] with the new tokens; every index array int32
+ * or int64.  max_q_len is the largest of q_seq_len; 1 selects the form for single tokens.  Rows of no sequence are not
+ * written, queries without a key get zeros, pages without a visible token are not looked at.  softcap > 0: scores become
+ * softcap * tanh(score * sm_scale / softcap).  hq / hkv <= 128, head sizes multiples of 8 up to 128, fp16 / bf16,
+ * sm_scale > 0, rows of q, out and the caches 16-byte aligned.  The reference has the window without sinks
+ * (python/dlBLAS/dlblas/kernels/paged_attention.py:421-424, 447). */
+int dlb_sink_attention(const void* q, const void* k_cache, const void* v_cache, void* out, const void* block_table,
+                       const void* q_start_loc, const void* q_seq_len, const void* kv_seq_len, int64_t batch,
+                       int64_t total_q_tokens, int64_t max_q_len, int64_t hq, int64_t hkv, int64_t head_dim,
+                       int64_t head_dim_v, int64_t page_size, int64_t num_pages, int64_t max_pages, int64_t q_stride_t,
+                       int64_t q_stride_h, int64_t o_stride_t, int64_t o_stride_h, int64_t k_stride_page,
+                       int64_t k_stride_slot, int64_t k_stride_head, int64_t v_stride_page, int64_t v_stride_slot,
+                       int64_t v_stride_head, int64_t bt_stride, int table_is_int64, int start_is_int64,
+                       int qlen_is_int64, int kvlen_is_int64, int64_t window, int64_t sinks, float sm_scale,
+                       float softcap, int dtype, int32_t* status, void* stream);
+
+/* Decode attention (one token per sequence) of groups that share a prefix, read once for the group: token b sees the
+ * prefix of its group, then its own tokens.  q [batch, hq, head_dim], out [batch, hq, head_dim_v]; group g is the
+ * sequences group_start[g] .. group_start[g + 1] - 1 (group_start [groups + 1]), its prefix the first prefix_len[g] tokens
+ * of row g of prefix_table [groups, prefix_max_pages]; a sequence's own tokens are the first kv_seq_len[b] of row b of
+ * block_table [batch, max_pages].  `chunk` (a multiple of 64) tokens of a prefix go to a split; `partial` is a workspace
+ * of dlb_shared_prefix_workspace_floats(batch, hq, larger head size, ceil(prefix_max_pages * page_size / chunk)) fp32,
+ * 16-byte aligned, in use until the call's work on the stream is done.  Two launches.  Everything else as for
+ * dlb_sink_attention.  No counterpart in the reference. */
+int64_t dlb_shared_prefix_workspace_floats(int64_t tokens, int64_t hq, int64_t head_dim, int64_t splits);
+int dlb_shared_prefix_attention(const void* q, const void* k_cache, const void* v_cache, void* out,
+                                const void* prefix_table, const void* prefix_len, const void* group_start,
+                                const void* block_table, const void* kv_seq_len, float* partial, int64_t batch,
+                                int64_t groups, int64_t hq, int64_t hkv, int64_t head_dim, int64_t head_dim_v,
+                                int64_t page_size, int64_t num_pages, int64_t prefix_max_pages, int64_t max_pages,
+                                int64_t q_stride_t, int64_t q_stride_h, int64_t o_stride_t, int64_t o_stride_h,
+                                int64_t k_stride_page, int64_t k_stride_slot, int64_t k_stride_head,
+                                int64_t v_stride_page, int64_t v_stride_slot, int64_t v_stride_head, int64_t pt_stride,
+                                int64_t bt_stride, int prefix_table_is_int64, int prefix_len_is_int64,
+                                int group_start_is_int64, int table_is_int64, int kvlen_is_int64, int64_t chunk,
+                                float sm_scale, float softcap, int dtype, int32_t* status, void* stream);
 
 /* rms_norm with optional residual add.  new_x = x + residual in the storage dtype (written to
  * out_residual when given); out = w * (new_x * rsqrt(mean(new_x^2) + eps)).  weight_after_cast = 0
