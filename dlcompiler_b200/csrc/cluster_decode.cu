@@ -12,10 +12,14 @@
 // HBM-bound, about 4 FLOP per byte.  The keys that a sequence can see are bounded by the window, so a cluster of at most
 // 8 CTAs is split enough and no partial result leaves the SMs; that saves the second launch and the workspace which a
 // split over an unbounded length needs.  A tile is 64 keys.  One producer lane per box issues TMA tile loads into a
-// 3-stage ring; at the ends of a range 16-row boxes fetch only what some key of the range needs, so that 4 sinks cost
+// 2-stage ring; at the ends of a range 16-row boxes fetch only what some key of the range needs, so that 4 sinks cost
 // 16 rows and not 64, and pages that hold no visible key are not looked at (a cache that drops tokens behind the
-// window may have reused them).  Four consumer warps own 16 keys of a tile each: mma.sync m16n8k16 with the q-heads
-// of the kv head as the M rows.
+// window may have reused them).  Four consumer warps own 16 keys of a tile each and compute S^T = K Q^T and O^T += V^T P
+// with mma.sync m16n8k16: keys (columns of V) are the 16 rows, eight q-heads of the kv head the 8 columns, so that 4 or 8
+// heads do not leave three quarters or half of the rows empty.  Against q-heads as rows this halves instructions and
+// accumulators, which lets three CTAs with two stages share an SM in place of two with three: 64 sequences with a window of
+// 4096, 8 kv heads, 128 columns: 202 -> 182 us (5.9 TB/s); 256 sequences of 16 to 512 own tokens and 8 pieces of a prefix:
+// 98 -> 58 us.
 #include <math_constants.h>
 
 #include "cluster_decode.cuh"
@@ -26,19 +30,21 @@ namespace cd {
 constexpr int TILE = 64;
 constexpr int CONSUMERS = 4;
 constexpr int THREADS = 32 * (CONSUMERS + 1);
-constexpr int STAGES = 3;
+constexpr int STAGES = 2;
 constexpr int EDGE_ROWS = 16;
 constexpr int MAX_CLUSTER = 8;
-template <int D> struct Layout {
+constexpr float RESCALE_THRESHOLD = 8.0f;                   // log2 units: P stays below 2^8, well inside fp16
+template <int D, int NH> struct Layout {
+  static constexpr int HEADS = 8 * NH;                      // q-heads to a CTA
   static constexpr int HALF_BYTES = TILE * 128;             // one 64-key x 64-column swizzled box
   static constexpr int BOXES = D / 64;
   static constexpr int KV_BYTES = BOXES * HALF_BYTES;
   static constexpr int STAGE_BYTES = 2 * KV_BYTES;
   static constexpr int RING = STAGES * STAGE_BYTES;
-  // after the loop the ring holds the warps' results and the CTA's
-  static constexpr int RED_FLOATS = CONSUMERS * 16 * (D + 2);
-  static constexpr int JOIN_FLOATS = 16 * (D + 2);
-  static constexpr int RESULTS = (RED_FLOATS + JOIN_FLOATS) * 4;
+  // after the loop the ring holds the warps' results and the CTA's, rows of PITCH floats (4 more than D, so that the lanes
+  // of a store, 8 columns of 4 heads, fall on 32 banks)
+  static constexpr int PITCH = D + 4;
+  static constexpr int RESULTS = (CONSUMERS + 1) * HEADS * (PITCH + 2) * 4;
   static constexpr int CTRL = RING > RESULTS ? RING : RESULTS;
   static constexpr int SMEM = CTRL + 128 + 1024;            // 1 KiB to align the ring
 };
@@ -47,23 +53,53 @@ template <int D> struct Layout {
 __device__ __forceinline__ void cluster_barrier() {
   asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }
-__device__ __forceinline__ float peer_load(uint32_t smem_addr, int rank) {
+__device__ __forceinline__ uint32_t peer_address(uint32_t smem_addr, int rank) {
   uint32_t at;
-  float v;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_addr), "r"(rank));
+  return at;
+}
+__device__ __forceinline__ float peer_load(uint32_t at) {
+  float v;
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
   return v;
 }
+__device__ __forceinline__ float4 peer_load4(uint32_t at) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
 
-template <typename T, int D, bool CAP, bool PREFIX>
-__global__ void __launch_bounds__(cd::THREADS, 2)
+// One running result (m, l, four columns) takes in another.
+struct Joined {
+  float m = -INFINITY, l = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  __device__ __forceinline__ void add(float pm, float pl, const float4& po) {
+    if (pm == -CUDART_INF_F) return;                        // a piece without keys
+    const float top = fmaxf(m, pm);
+    const float a = m == -CUDART_INF_F ? 0.f : fast_exp2(m - top), b = fast_exp2(pm - top);
+    m = top;
+    l = l * a + pl * b;
+    o.x = o.x * a + po.x * b;
+    o.y = o.y * a + po.y * b;
+    o.z = o.z * a + po.z * b;
+    o.w = o.w * a + po.w * b;
+  }
+};
+
+template <typename T, int D, int NH, bool CAP, bool PREFIX>
+__global__ void __launch_bounds__(cd::THREADS, NH == 1 ? 3 : 2)
 cluster_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
                       const __grid_constant__ CUtensorMap edge_k, const __grid_constant__ CUtensorMap edge_v,
                       const __grid_constant__ ClusterDecodeParams p) {
   using namespace cd;
-  using L = Layout<D>;
+  using L = Layout<D, NH>;
   constexpr int KSTEPS = D / 16;
-  constexpr int NT = D / 8;
+  constexpr int MT = D / 16;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_u32(smem_raw);
   uint8_t* smem = smem_raw + (((raw_addr + 1023u) & ~1023u) - raw_addr);
@@ -74,7 +110,7 @@ cluster_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
 
   const int rank = blockIdx.x, cluster = gridDim.x;
   const int kvh = blockIdx.y % p.hkv;
-  const int hblk = blockIdx.y / p.hkv;                       // block of 16 q-heads of the kv head
+  const int hblk = blockIdx.y / p.hkv;                       // block of q-heads of the kv head
   const int b = blockIdx.z;
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -114,15 +150,23 @@ cluster_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
   }
   __syncthreads();
 
-  const int rows_valid = min(16, p.group - hblk * 16);       // q-heads of this CTA
-  const int head0 = kvh * p.group + hblk * 16;
-  float m_run[2] = {-CUDART_INF_F, -CUDART_INF_F};
-  float l_run[2] = {0.f, 0.f};
-  float oacc[NT][4];
+  const int rows_valid = min(L::HEADS, p.group - hblk * L::HEADS);   // q-heads of this CTA
+  const int head0 = kvh * p.group + hblk * L::HEADS;
+  // a thread's heads: 8 n + (lane & 3) * 2 and the next
+  float m_run[NH][2], l_run[NH][2];
+  float oacc[NH][MT][4];
 #pragma unroll
-  for (int t = 0; t < NT; ++t)
+  for (int n = 0; n < NH; ++n) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) oacc[t][j] = 0.f;
+    for (int e = 0; e < 2; ++e) {
+      m_run[n][e] = -CUDART_INF_F;
+      l_run[n][e] = 0.f;
+    }
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) oacc[n][t][j] = 0.f;
+  }
 
   if (warp == CONSUMERS) {
     // ------------------------------ producer ------------------------------
@@ -187,20 +231,22 @@ cluster_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
     }
   } else {
     // ------------------------------ consumers ------------------------------
-    const int r0 = lane >> 2;        // fragment row (q-head) 0..7, second row is r0 + 8
-    const int cq = (lane & 3) * 2;   // fragment column pair
-    uint32_t qf[KSTEPS][4];
+    // Q^T as the B operand: head lane / 4 (of each block of 8), columns (lane & 3) * 2 of every 8
+    uint32_t qf[NH][KSTEPS][2];
     {
       const T* qb = reinterpret_cast<const T*>(p.q) + row * p.q_st;
 #pragma unroll
-      for (int ks = 0; ks < KSTEPS; ++ks) {
+      for (int n = 0; n < NH; ++n) {
+        const int r = n * 8 + (lane >> 2);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int r = r0 + (j & 1) * 8;
-          const int col = ks * 16 + cq + (j >> 1) * 8;
-          uint32_t v = 0;
-          if (r < rows_valid && col < p.dk) v = *reinterpret_cast<const uint32_t*>(qb + (int64_t)(head0 + r) * p.q_sh + col);
-          qf[ks][j] = v;
+        for (int ks = 0; ks < KSTEPS; ++ks) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int col = ks * 16 + (lane & 3) * 2 + j * 8;
+            uint32_t v = 0;
+            if (r < rows_valid && col < p.dk) v = *reinterpret_cast<const uint32_t*>(qb + (int64_t)(head0 + r) * p.q_sh + col);
+            qf[n][ks][j] = v;
+          }
         }
       }
     }
@@ -249,153 +295,147 @@ cluster_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
         __syncwarp();
       }
 
-      // ---- S = Q K^T for this warp's 16 keys ----
-      float sacc[2][4];
+      // ---- S^T = K Q^T: this warp's 16 keys by 8 NH heads ----
+      float sacc[NH][4];
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+      for (int n = 0; n < NH; ++n)
 #pragma unroll
-        for (int u = 0; u < 4; ++u) sacc[j][u] = 0.f;
+        for (int u = 0; u < 4; ++u) sacc[n][u] = 0.f;
 #pragma unroll
       for (int ks = 0; ks < KSTEPS; ++ks) {
-        const int key = warp * 16 + (mat >> 1) * 8 + mrow;
-        const int ch = ks * 2 + (mat & 1);
-        const uint32_t addr = kbase + (ch >> 3) * L::HALF_BYTES + key * 128 + (((ch & 7) ^ (key & 7)) << 4);
-        uint32_t b00, b01, b10, b11;
-        ldmatrix_x4(addr, b00, b01, b10, b11);
-        mma_16816<T>(sacc[0], qf[ks], b00, b01);
-        mma_16816<T>(sacc[1], qf[ks], b10, b11);
+        const int key = warp * 16 + (mat & 1) * 8 + mrow;
+        const int ch = ks * 2 + (mat >> 1);
+        uint32_t a[4];
+        ldmatrix_x4(kbase + (ch >> 3) * L::HALF_BYTES + key * 128 + (((ch & 7) ^ (key & 7)) << 4), a[0], a[1], a[2], a[3]);
+#pragma unroll
+        for (int n = 0; n < NH; ++n) mma_16816<T>(sacc[n], a, qf[n][ks][0], qf[n][ks][1]);
       }
 
-      // ---- scale, soft-cap, mask, running maximum (base-2 domain) ----
-      float mx[2] = {-CUDART_INF_F, -CUDART_INF_F};
+      // ---- scale, soft-cap, mask (base-2 domain); the reference maximum is raised when a score passes it by 2^8 ----
+      bool grow = false;
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
+      for (int n = 0; n < NH; ++n) {
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-          float v = sacc[j][u];
+          float v = sacc[n][u];
           if (CAP) v = cap_out * tanhf(v * cap_in);
           else v *= scale2;
           if (partly) {
-            const int key = key0 + j * 8 + cq + (u & 1);
+            const int key = key0 + (lane >> 2) + (u >> 1) * 8;
             v = (key >= from && key < to) ? v : -CUDART_INF_F;
           }
-          sacc[j][u] = v;
-          mx[u >> 1] = fmaxf(mx[u >> 1], v);
+          sacc[n][u] = v;
+          // m_run -inf: any score that is not -inf itself
+          grow |= v > m_run[n][u & 1] + RESCALE_THRESHOLD;
         }
       }
+      if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
-        mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
-      }
-      float alpha[2];
-      bool grew = false;
+        for (int n = 0; n < NH; ++n) {
+          float alpha[2];
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const float m_new = fmaxf(m_run[r], mx[r]);
-        alpha[r] = (m_new == -CUDART_INF_F) ? 1.f : fast_exp2(m_run[r] - m_new);
-        grew |= (m_new > m_run[r]) && (m_run[r] != -CUDART_INF_F);
-        m_run[r] = m_new;
-      }
-      float psum[2] = {0.f, 0.f};
-      uint32_t pf[4];
-      {
-        float pv[2][4];
+          for (int e = 0; e < 2; ++e) {
+            float mx = fmaxf(sacc[n][e], sacc[n][e + 2]);
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            const float mref = m_run[u >> 1];
-            const float e = (mref == -CUDART_INF_F) ? 0.f : fast_exp2(sacc[j][u] - mref);
-            pv[j][u] = e;
-            psum[u >> 1] += e;
+            for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+            mx = fmaxf(mx, m_run[n][e]);
+            alpha[e] = m_run[n][e] == -CUDART_INF_F ? 0.f : fast_exp2(m_run[n][e] - mx);
+            m_run[n][e] = mx;
+            l_run[n][e] *= alpha[e];
           }
-        pf[0] = pack_pair<T>(pv[0][0], pv[0][1]);
-        pf[1] = pack_pair<T>(pv[0][2], pv[0][3]);
-        pf[2] = pack_pair<T>(pv[1][0], pv[1][1]);
-        pf[3] = pack_pair<T>(pv[1][2], pv[1][3]);
-      }
 #pragma unroll
-      for (int r = 0; r < 2; ++r) l_run[r] = l_run[r] * alpha[r] + psum[r];
-      if (__any_sync(0xffffffffu, grew)) {
-#pragma unroll
-        for (int tt = 0; tt < NT; ++tt) {
-          oacc[tt][0] *= alpha[0];
-          oacc[tt][1] *= alpha[0];
-          oacc[tt][2] *= alpha[1];
-          oacc[tt][3] *= alpha[1];
+          for (int tt = 0; tt < MT; ++tt) {
+            oacc[n][tt][0] *= alpha[0];
+            oacc[n][tt][1] *= alpha[1];
+            oacc[n][tt][2] *= alpha[0];
+            oacc[n][tt][3] *= alpha[1];
+          }
         }
+      }
+      uint32_t pf[NH][2];
+#pragma unroll
+      for (int n = 0; n < NH; ++n) {
+        float e[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const float mref = m_run[n][u & 1];
+          e[u] = mref == -CUDART_INF_F ? 0.f : fast_exp2(sacc[n][u] - mref);
+          l_run[n][u & 1] += e[u];
+        }
+        pf[n][0] = transpose_8x8(pack_pair<T>(e[0], e[1]));
+        pf[n][1] = transpose_8x8(pack_pair<T>(e[2], e[3]));
       }
 
-      // ---- O += P V ----
+      // ---- O^T += V^T P ----
 #pragma unroll
-      for (int n = 0; n < D / 16; ++n) {
-        const int key = warp * 16 + (mat & 1) * 8 + mrow;
-        const int ch = n * 2 + (mat >> 1);
-        const uint32_t addr = vbase + (ch >> 3) * L::HALF_BYTES + key * 128 + (((ch & 7) ^ (key & 7)) << 4);
-        uint32_t v00, v01, v10, v11;
-        ldmatrix_x4_trans(addr, v00, v01, v10, v11);
-        mma_16816<T>(oacc[2 * n], pf, v00, v01);
-        mma_16816<T>(oacc[2 * n + 1], pf, v10, v11);
+      for (int m = 0; m < MT; ++m) {
+        const int key = warp * 16 + (mat >> 1) * 8 + mrow;
+        const int ch = m * 2 + (mat & 1);
+        uint32_t a[4];
+        ldmatrix_x4_trans(vbase + (ch >> 3) * L::HALF_BYTES + key * 128 + (((ch & 7) ^ (key & 7)) << 4), a[0], a[1], a[2],
+                          a[3]);
+#pragma unroll
+        for (int n = 0; n < NH; ++n) mma_16816<T>(oacc[n][m], a, pf[n][0], pf[n][1]);
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty_bar[s]);
     }
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {    // each lane summed its own 4 keys of a row
-      l_run[r] += __shfl_xor_sync(0xffffffffu, l_run[r], 1);
-      l_run[r] += __shfl_xor_sync(0xffffffffu, l_run[r], 2);
-    }
+    for (int n = 0; n < NH; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)    // each lane summed its own keys
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) l_run[n][e] += __shfl_xor_sync(0xffffffffu, l_run[n][e], o);
   }
 
   // ------------------------------ join the warps ------------------------------
   __syncthreads();   // every load has been consumed: the ring can be reused
-  float* red_o = reinterpret_cast<float*>(smem);             // [warps][16][D]
-  float* red_m = red_o + CONSUMERS * 16 * D;                 // [warps][16]
-  float* red_l = red_m + CONSUMERS * 16;
-  float* join_o = red_l + CONSUMERS * 16;                    // [16][D], the CTA's result
-  float* join_m = join_o + 16 * D;
-  float* join_l = join_m + 16;
+  constexpr int H = L::HEADS, PITCH = L::PITCH, QUADS = D / 4;
+  float* red_o = reinterpret_cast<float*>(smem);             // [warps + 1][H][PITCH], the last one the CTA's
+  float* red_m = red_o + (CONSUMERS + 1) * H * PITCH;        // [warps + 1][H]
+  float* red_l = red_m + (CONSUMERS + 1) * H;
   if (warp < CONSUMERS) {
-    const int r0 = lane >> 2;
-    const int cq = (lane & 3) * 2;
 #pragma unroll
-    for (int tt = 0; tt < NT; ++tt) {
-      float2* o0 = reinterpret_cast<float2*>(red_o + (warp * 16 + r0) * D + tt * 8 + cq);
-      float2* o1 = reinterpret_cast<float2*>(red_o + (warp * 16 + r0 + 8) * D + tt * 8 + cq);
-      *o0 = make_float2(oacc[tt][0], oacc[tt][1]);
-      *o1 = make_float2(oacc[tt][2], oacc[tt][3]);
-    }
-    if ((lane & 3) == 0) {
-      red_m[warp * 16 + r0] = m_run[0];
-      red_m[warp * 16 + r0 + 8] = m_run[1];
-      red_l[warp * 16 + r0] = l_run[0];
-      red_l[warp * 16 + r0 + 8] = l_run[1];
+    for (int n = 0; n < NH; ++n) {
+      const int h = n * 8 + (lane & 3) * 2;
+      float* o = red_o + (warp * H + h) * PITCH + (lane >> 2);
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        o[m * 16] = oacc[n][m][0];
+        o[PITCH + m * 16] = oacc[n][m][1];
+        o[m * 16 + 8] = oacc[n][m][2];
+        o[PITCH + m * 16 + 8] = oacc[n][m][3];
+      }
+      if (lane < 4) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          red_m[warp * H + h + e] = m_run[n][e];
+          red_l[warp * H + h + e] = l_run[n][e];
+        }
+      }
     }
   }
   __syncthreads();
   T* out = reinterpret_cast<T*>(p.out) + row * p.o_st;
-  for (int idx = threadIdx.x; idx < rows_valid * D; idx += THREADS) {
-    const int r = idx / D;
-    const int d = idx - r * D;
-    float m = -CUDART_INF_F;
+  auto store = [&](int r, int d, const Joined& j) {
+    if (d >= p.dv) return;
+    const float inv = j.l > 0.f ? 1.f / j.l : 0.f;
+    typename Elem<T>::T2 v[2] = {Elem<T>::from_f2(j.o.x * inv, j.o.y * inv), Elem<T>::from_f2(j.o.z * inv, j.o.w * inv)};
+    *reinterpret_cast<uint2*>(out + (int64_t)(head0 + r) * p.o_sh + d) = *reinterpret_cast<const uint2*>(v);
+  };
+  for (int idx = threadIdx.x; idx < rows_valid * QUADS; idx += THREADS) {
+    const int r = idx / QUADS, d = idx % QUADS * 4;
+    Joined j;
 #pragma unroll
-    for (int w = 0; w < CONSUMERS; ++w) m = fmaxf(m, red_m[w * 16 + r]);
-    float acc = 0.f, l = 0.f;
-#pragma unroll
-    for (int w = 0; w < CONSUMERS; ++w) {
-      const float mw = red_m[w * 16 + r];
-      const float sc = (mw == -CUDART_INF_F) ? 0.f : fast_exp2(mw - m);
-      acc += red_o[(w * 16 + r) * D + d] * sc;
-      l += red_l[w * 16 + r] * sc;
-    }
+    for (int w = 0; w < CONSUMERS; ++w)
+      j.add(red_m[w * H + r], red_l[w * H + r], *reinterpret_cast<const float4*>(red_o + (w * H + r) * PITCH + d));
     if (!PREFIX && cluster == 1) {
-      if (d < p.dv) out[(int64_t)(head0 + r) * p.o_sh + d] = Elem<T>::from_f(l > 0.f ? acc / l : 0.f);
+      store(r, d, j);
     } else {
-      join_o[idx] = acc;
+      *reinterpret_cast<float4*>(red_o + (CONSUMERS * H + r) * PITCH + d) = j.o;
       if (d == 0) {
-        join_m[r] = m;
-        join_l[r] = l;
+        red_m[CONSUMERS * H + r] = j.m;
+        red_l[CONSUMERS * H + r] = j.l;
       }
     }
   }
@@ -404,49 +444,51 @@ cluster_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
   // ------------------------------ join the cluster (and the prefix) ------------------------------
   if (cluster > 1) cluster_barrier();
   else __syncthreads();
-  const uint32_t addr_o = smem_u32(join_o), addr_m = smem_u32(join_m), addr_l = smem_u32(join_l);
+  const uint32_t at_o = smem_u32(red_o + CONSUMERS * H * PITCH), at_m = smem_u32(red_m + CONSUMERS * H),
+                 at_l = smem_u32(red_l + CONSUMERS * H);
   const int ext = PREFIX ? *ext_splits : 0;
-  for (int idx = rank * THREADS + threadIdx.x; idx < rows_valid * D; idx += cluster * THREADS) {
-    const int r = idx / D;
-    const int d = idx - r * D;
-    float m = -CUDART_INF_F;
-    for (int c = 0; c < cluster; ++c) m = fmaxf(m, peer_load(addr_m + r * 4, c));
-    const int64_t prow = row * p.hq + head0 + r, rows_all = p.tokens * p.hq;
-    if constexpr (PREFIX)
-      for (int s = 0; s < ext; ++s) m = fmaxf(m, p.prefix.ml[s * rows_all + prow].x);
-    float acc = 0.f, l = 0.f;
-    for (int c = 0; c < cluster; ++c) {
-      const float mc = peer_load(addr_m + r * 4, c);
-      const float sc = (mc == -CUDART_INF_F) ? 0.f : fast_exp2(mc - m);
-      acc += peer_load(addr_o + idx * 4, c) * sc;
-      l += peer_load(addr_l + r * 4, c) * sc;
-    }
+  const int per_rank = (rows_valid * QUADS + cluster - 1) / cluster;
+  const int idx_hi = min(rows_valid * QUADS, (rank + 1) * per_rank);
+  for (int idx = rank * per_rank + threadIdx.x; idx < idx_hi; idx += THREADS) {
+    const int r = idx / QUADS, d = idx % QUADS * 4;
+    Joined j;
+    for (int c = 0; c < cluster; ++c)
+      j.add(peer_load(peer_address(at_m + r * 4, c)), peer_load(peer_address(at_l + r * 4, c)),
+            peer_load4(peer_address(at_o + (r * PITCH + d) * 4, c)));
     if constexpr (PREFIX) {
-      for (int s = 0; s < ext; ++s) {
-        const float2 ml = p.prefix.ml[s * rows_all + prow];
-        const float sc = (ml.x == -CUDART_INF_F) ? 0.f : fast_exp2(ml.x - m);
-        acc += p.prefix.o[(s * rows_all + prow) * D + d] * sc;
-        l += ml.y * sc;
+      const int64_t prow = row * p.hq + head0 + r, rows_all = p.tokens * p.hq;
+      for (int s = 0; s < ext; s += 4) {
+        float2 ml[4];
+        float4 o[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int64_t k = min(s + u, ext - 1) * rows_all + prow;
+          ml[u] = p.prefix.ml[k];
+          o[u] = *reinterpret_cast<const float4*>(p.prefix.o + k * D + d);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (s + u < ext) j.add(ml[u].x, ml[u].y, o[u]);
       }
     }
-    if (d < p.dv) out[(int64_t)(head0 + r) * p.o_sh + d] = Elem<T>::from_f(l > 0.f ? acc / l : 0.f);
+    store(r, d, j);
   }
   if (cluster > 1) cluster_barrier();    // a CTA's shared memory stays until its peers have read it
 }
 
 // CTAs to a (sequence, kv head): doubled while the launch leaves SMs without work, down to two tiles a CTA, and up to four
-// waves of two CTAs per SM while a CTA keeps eight tiles.
-static int pick_cluster(int64_t pairs, int64_t tiles) {
+// waves of the CTAs that are resident while a CTA keeps eight tiles.
+static int pick_cluster(int64_t pairs, int64_t tiles, int resident) {
   int c = 1;
-  const int64_t slots = 2 * sm_count(current_device());
+  const int64_t slots = resident * sm_count(current_device());
   while (c < cd::MAX_CLUSTER && ((pairs * c < slots && tiles >= 4 * c) || (pairs * c < 4 * slots && tiles >= 16 * c))) c *= 2;
   return c;
 }
 
-template <typename T, int D, bool CAP, bool PREFIX>
+template <typename T, int D, int NH, bool CAP, bool PREFIX>
 static int launch_cluster(const CUtensorMap (&maps)[4], const ClusterDecodeParams& p, int cluster, cudaStream_t stream) {
-  auto kern = cluster_decode_kernel<T, D, CAP, PREFIX>;
-  constexpr int SMEM = cd::Layout<D>::SMEM;
+  auto kern = cluster_decode_kernel<T, D, NH, CAP, PREFIX>;
+  constexpr int SMEM = cd::Layout<D, NH>::SMEM;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
   if (e != cudaSuccess) {
     set_last_error("cluster_decode: cannot raise dynamic shared memory: %s", cudaGetErrorString(e));
@@ -457,7 +499,7 @@ static int launch_cluster(const CUtensorMap (&maps)[4], const ClusterDecodeParam
   attr[0].val.clusterDim.x = cluster;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(cluster, p.hkv * ((p.group + 15) / 16), p.batch);
+  cfg.gridDim = dim3(cluster, p.hkv * ((p.group + 8 * NH - 1) / (8 * NH)), p.batch);
   cfg.blockDim = dim3(cd::THREADS);
   cfg.dynamicSmemBytes = SMEM;
   cfg.stream = stream;
@@ -471,14 +513,25 @@ static int launch_cluster(const CUtensorMap (&maps)[4], const ClusterDecodeParam
   }
   return DLB_OK;
 }
-template <typename T, int D>
+template <typename T, int D, int NH>
 static int launch_cluster(const CUtensorMap (&maps)[4], const ClusterDecodeParams& p, int cluster, cudaStream_t stream) {
   const bool cap = p.softcap > 0.f;
   if (p.prefix.o != nullptr)
-    return cap ? launch_cluster<T, D, true, true>(maps, p, cluster, stream)
-               : launch_cluster<T, D, false, true>(maps, p, cluster, stream);
-  return cap ? launch_cluster<T, D, true, false>(maps, p, cluster, stream)
-             : launch_cluster<T, D, false, false>(maps, p, cluster, stream);
+    return cap ? launch_cluster<T, D, NH, true, true>(maps, p, cluster, stream)
+               : launch_cluster<T, D, NH, false, true>(maps, p, cluster, stream);
+  return cap ? launch_cluster<T, D, NH, true, false>(maps, p, cluster, stream)
+             : launch_cluster<T, D, NH, false, false>(maps, p, cluster, stream);
+}
+template <typename T>
+static int launch_cluster(const CUtensorMap (&maps)[4], const ClusterDecodeParams& p, int width, int64_t key_bound,
+                          cudaStream_t stream) {
+  // up to 8 heads to a kv head fill one block of the B operand; with more a CTA takes 16
+  const bool narrow = p.group <= 8;
+  const int64_t pairs = (int64_t)p.batch * p.hkv * (narrow ? 1 : (p.group + 15) / 16);
+  const int cluster = pick_cluster(pairs, (key_bound + cd::TILE - 1) / cd::TILE, narrow ? 3 : 2);
+  if (narrow)
+    return width == 128 ? launch_cluster<T, 128, 1>(maps, p, cluster, stream) : launch_cluster<T, 64, 1>(maps, p, cluster, stream);
+  return width == 128 ? launch_cluster<T, 128, 2>(maps, p, cluster, stream) : launch_cluster<T, 64, 2>(maps, p, cluster, stream);
 }
 
 int launch_cluster_decode(const ClusterDecodeParams& p, const void* k_cache, const void* v_cache, int64_t k_stride_page,
@@ -497,13 +550,8 @@ int launch_cluster_decode(const ClusterDecodeParams& p, const void* k_cache, con
                                    k ? k_stride_head : v_stride_head, i < 2 ? full : cd::EDGE_ROWS);
     if (rc != DLB_OK) return rc;
   }
-  const int64_t pairs = (int64_t)p.batch * p.hkv * ((p.group + 15) / 16);
-  const int cluster = pick_cluster(pairs, (key_bound + cd::TILE - 1) / cd::TILE);
-  if (dtype == DLB_DTYPE_BF16)
-    return width == 128 ? launch_cluster<__nv_bfloat16, 128>(maps, p, cluster, stream)
-                        : launch_cluster<__nv_bfloat16, 64>(maps, p, cluster, stream);
-  return width == 128 ? launch_cluster<__half, 128>(maps, p, cluster, stream)
-                      : launch_cluster<__half, 64>(maps, p, cluster, stream);
+  return dtype == DLB_DTYPE_BF16 ? launch_cluster<__nv_bfloat16>(maps, p, width, key_bound, stream)
+                                 : launch_cluster<__half>(maps, p, width, key_bound, stream);
 }
 
 }  // namespace dlb

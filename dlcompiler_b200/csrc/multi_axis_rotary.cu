@@ -38,15 +38,20 @@ template <typename T, int VEC> struct alignas(sizeof(T) * VEC) ElemVec {
   T v[VEC];
 };
 
-// A CTA takes TOK tokens with THREADS / TOK threads each; a thread keeps its column (VEC elements of the lower half
-// and the matching ones of the upper half, or VEC columns behind them) and its token's cos / sin and walks the heads.
+// A CTA forms the cos / sin of TOK tokens in shared memory, then its threads walk the tokens' items: VEC columns of a head's
+// lower half and the matching ones of the upper half, or two vectors of the columns behind them.
 template <typename T, int VEC, int TOK>
-__global__ void __launch_bounds__(mar::THREADS) multi_axis_rotary_kernel(const __grid_constant__ MultiAxisParams p) {
+__global__ void __launch_bounds__(mar::THREADS, VEC == 8 ? 6 : 8) multi_axis_rotary_kernel(const __grid_constant__ MultiAxisParams p) {
   using V = ElemVec<T, VEC>;
-  constexpr int G = mar::THREADS / TOK;
-  __shared__ float s_cos[TOK * mar::MAX_HALF], s_sin[TOK * mar::MAX_HALF];
+  __shared__ __align__(16) float s_cos[TOK * mar::MAX_HALF], s_sin[TOK * mar::MAX_HALF];
   const int64_t t0 = (int64_t)blockIdx.x * TOK;
   const int ntok = (int)min((int64_t)TOK, p.tokens - t0);
+  const int hv = p.half / VEC, rv = p.rest / VEC;    // items of the pairs; vectors behind them, two to an item
+  // Item i's values lie in quads, quad g of all items side by side, so that lanes next to one another read 16 bytes apart
+  auto place = [&](int tl, int f) {
+    const int i = f / VEC, j = f % VEC;
+    return tl * mar::MAX_HALF + (VEC < 4 ? f : (j >> 2) * hv * 4 + i * 4 + (j & 3));
+  };
   for (int idx = threadIdx.x; idx < ntok * p.half; idx += mar::THREADS) {
     const int tl = TOK == 1 ? 0 : idx / p.half;
     const int f = idx - tl * p.half;
@@ -59,63 +64,63 @@ __global__ void __launch_bounds__(mar::THREADS) multi_axis_rotary_kernel(const _
     const float off = (float)(part - (double)x) * 3.14159265358979f;
     float s, c;
     sincospif(x, &s, &c);
-    s_cos[tl * mar::MAX_HALF + f] = fmaf(-s, off, c);
-    s_sin[tl * mar::MAX_HALF + f] = fmaf(c, off, s) * p.sign;
+    s_cos[place(tl, f)] = fmaf(-s, off, c);
+    s_sin[place(tl, f)] = fmaf(c, off, s) * p.sign;
   }
   __syncthreads();
-  const int tl = threadIdx.x / G, lt = threadIdx.x % G;
-  if (tl >= ntok) return;
-  const int hv = p.half / VEC;                       // pair items of a row, then p.rest / VEC copies
-  const int width = hv + p.rest / VEC;
-  const int rows = max(G / width, 1), r0 = width <= G ? lt / width : 0;
-  if (r0 >= rows) return;
-  const int heads = p.hq + p.hk;
-  const int64_t t = t0 + tl;
-  const T* q = reinterpret_cast<const T*>(p.q) + t * p.q_st;
-  const T* k = reinterpret_cast<const T*>(p.k) + t * p.k_st;
-  T* qo = reinterpret_cast<T*>(p.qo) + t * p.qo_st;
-  T* ko = reinterpret_cast<T*>(p.ko) + t * p.ko_st;
-  for (int i = width <= G ? lt - r0 * width : lt; i < width; i += G) {
-    if (i < hv) {
-      float c[VEC], s[VEC];
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        c[j] = s_cos[tl * mar::MAX_HALF + i * VEC + j];
-        s[j] = s_sin[tl * mar::MAX_HALF + i * VEC + j];
-      }
-#pragma unroll 4
-      for (int h = r0; h < heads; h += rows) {
-        const bool is_q = h < p.hq;
-        const T* src = (is_q ? q + (int64_t)h * p.q_sh : k + (int64_t)(h - p.hq) * p.k_sh) + i * VEC;
-        T* dst = (is_q ? qo + (int64_t)h * p.qo_sh : ko + (int64_t)(h - p.hq) * p.ko_sh) + i * VEC;
-        const V lo = *reinterpret_cast<const V*>(src), hi = *reinterpret_cast<const V*>(src + p.half);
-        V olo, ohi;
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          const float a = Elem<T>::to_f(lo.v[j]), b = Elem<T>::to_f(hi.v[j]);
-          olo.v[j] = Elem<T>::from_f(fmaf(a, c[j], -b * s[j]));
-          ohi.v[j] = Elem<T>::from_f(fmaf(b, c[j], a * s[j]));
-        }
-        *reinterpret_cast<V*>(dst) = olo;
-        *reinterpret_cast<V*>(dst + p.half) = ohi;
-      }
+  const int width = hv + (rv + 1) / 2;
+  const int per_token = (p.hq + p.hk) * width;
+  for (int idx = threadIdx.x; idx < ntok * per_token; idx += mar::THREADS) {
+    const int tl = TOK == 1 ? 0 : idx / per_token;
+    const int rem = idx - tl * per_token;
+    const int h = rem / width;
+    const int i = rem - h * width;
+    const int64_t t = t0 + tl;
+    const T* src;
+    T* dst;
+    if (h < p.hq) {
+      src = reinterpret_cast<const T*>(p.q) + t * p.q_st + (int64_t)h * p.q_sh;
+      dst = reinterpret_cast<T*>(p.qo) + t * p.qo_st + (int64_t)h * p.qo_sh;
     } else {
-      const int col = 2 * p.half + (i - hv) * VEC;
-      for (int h = r0; h < heads; h += rows) {
-        const bool is_q = h < p.hq;
-        const T* src = is_q ? q + (int64_t)h * p.q_sh : k + (int64_t)(h - p.hq) * p.k_sh;
-        T* dst = is_q ? qo + (int64_t)h * p.qo_sh : ko + (int64_t)(h - p.hq) * p.ko_sh;
-        *reinterpret_cast<V*>(dst + col) = *reinterpret_cast<const V*>(src + col);
+      src = reinterpret_cast<const T*>(p.k) + t * p.k_st + (int64_t)(h - p.hq) * p.k_sh;
+      dst = reinterpret_cast<T*>(p.ko) + t * p.ko_st + (int64_t)(h - p.hq) * p.ko_sh;
+    }
+    if (i < hv) {
+      V lo = *reinterpret_cast<const V*>(src + i * VEC), hi = *reinterpret_cast<const V*>(src + p.half + i * VEC);
+      constexpr int QUAD = VEC < 4 ? 1 : 4;
+#pragma unroll
+      for (int g = 0; g < VEC / QUAD; ++g) {
+        float c[QUAD], s[QUAD];
+        const int at = tl * mar::MAX_HALF + (g * hv + i) * QUAD;
+        *reinterpret_cast<ElemVec<float, QUAD>*>(c) = *reinterpret_cast<const ElemVec<float, QUAD>*>(s_cos + at);
+        *reinterpret_cast<ElemVec<float, QUAD>*>(s) = *reinterpret_cast<const ElemVec<float, QUAD>*>(s_sin + at);
+#pragma unroll
+        for (int j = 0; j < QUAD; ++j) {
+          const float a = Elem<T>::to_f(lo.v[g * QUAD + j]), b = Elem<T>::to_f(hi.v[g * QUAD + j]);
+          lo.v[g * QUAD + j] = Elem<T>::from_f(fmaf(a, c[j], -b * s[j]));
+          hi.v[g * QUAD + j] = Elem<T>::from_f(fmaf(b, c[j], a * s[j]));
+        }
       }
+      *reinterpret_cast<V*>(dst + i * VEC) = lo;
+      *reinterpret_cast<V*>(dst + p.half + i * VEC) = hi;
+    } else {
+      const int col = 2 * p.half + (i - hv) * 2 * VEC;
+      const bool both = (i - hv) * 2 + 1 < rv;
+      const V a = *reinterpret_cast<const V*>(src + col);
+      V b;
+      if (both) b = *reinterpret_cast<const V*>(src + col + VEC);
+      *reinterpret_cast<V*>(dst + col) = a;
+      if (both) *reinterpret_cast<V*>(dst + col + VEC) = b;
     }
   }
 }
 
 template <typename T, int VEC> static int launch_multi_axis(const MultiAxisParams& p, cudaStream_t s) {
-  // Four tokens to a CTA give a thread several heads per cos / sin that it holds; one token to a CTA where there are
-  // few, so that the call spreads over the SMs, or where a token's columns need all the threads.
-  const int width = p.half / VEC + p.rest / VEC;
-  if (p.tokens > 4 * 148 && width <= mar::THREADS / 4)
+  // Four tokens to a CTA, one where there are so few that they would not cover the SMs.  CTAs per SM (what the registers
+  // are cut to): 16-byte items, 32768 tokens of 32 + 8 heads of 128 in bf16: 125.0 us at 4, 115.5 at 5, 108.7 at 6 (6.2
+  // TB/s), 109.8 at 8, where some values spill; 8-byte items, 9217 tokens of 16 + 16 heads of 80: 31.9 / 32.2 / 28.4 / 26.3.
+  // Eight tokens to a CTA: 111.2 and 31.0.
+  if (p.tokens > 4 * 148)
     multi_axis_rotary_kernel<T, VEC, 4><<<(unsigned)((p.tokens + 3) / 4), mar::THREADS, 0, s>>>(p);
   else
     multi_axis_rotary_kernel<T, VEC, 1><<<(unsigned)p.tokens, mar::THREADS, 0, s>>>(p);
