@@ -88,7 +88,7 @@ SIGNATURES = {
     "dlb_sink_attention": (c_int, [c_void_p] * 8 + [c_int64] * 21 + [c_int] * 4 + [c_int64] * 2 + [c_float] * 2 +
                            [c_int, c_void_p, c_void_p]),
     "dlb_shared_prefix_workspace_floats": (c_int64, [c_int64] * 4),
-    "dlb_shared_prefix_attention": (c_int, [c_void_p] * 10 + [c_int64] * 22 + [c_int] * 5 + [c_int64] + [c_float] * 2 +
+    "dlb_shared_prefix_attention": (c_int, [c_void_p] * 10 + [c_int64] * 22 + [c_int] * 5 + [c_int64] * 2 + [c_float] * 2 +
                                     [c_int, c_void_p, c_void_p]),
     "dlb_fill_kv_cache": (c_int, [c_void_p] * 8 + [c_int64] * 19 + [c_int] * 5 + [c_void_p, c_void_p, c_int, c_void_p]),
     "dlb_paged_decode_static": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
@@ -180,14 +180,13 @@ def stream_ptr(device=None) -> int:
 def require_cuda(*tensors: torch.Tensor) -> torch.device:
     dev = None
     for t in tensors:
-        if t is None:
+        if t is None or t.device == dev:
             continue
         if not t.is_cuda:
             raise AssertionError("dlcompiler_b200 ops run on CUDA tensors only (no CPU fallback)")
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
+        if dev is not None:
             raise AssertionError("all tensors must be on the same CUDA device")
+        dev = t.device
     return dev
 
 

@@ -25,6 +25,38 @@ static inline int make_tmap_tokens(CUtensorMap* out, const void* base, int64_t d
   return DLB_OK;
 }
 
+// Tensor map of a paged cache [pages, slots, heads, d] for boxes of `box_slots` rows of one head that land as 64 columns after 64
+// columns, box_slots rows of 128 bytes each.  With `whole` (a head size that is a multiple of 64) a box has all columns of its
+// rows: a 5-D map, loaded by tma_load_5d.  Otherwise one of 64 columns, loaded by tma_load_4d, and the copy engine fills the
+// columns past the head size with zeros.
+static inline int make_tmap_rows(CUtensorMap* out, const void* base, int64_t d, int64_t heads, int64_t slots, int64_t pages,
+                                 int64_t stride_page, int64_t stride_slot, int64_t stride_head, int box_slots, bool whole) {
+  if (!whole) return make_tmap_cache(out, base, d, heads, slots, pages, stride_page, stride_slot, stride_head, box_slots);
+  PFN_encodeTiled enc = get_encode_tiled();
+  DLB_CHECK_ARG(enc != nullptr, DLB_ERR_DRIVER, "cuTensorMapEncodeTiled is not available from the driver");
+  DLB_CHECK_ARG(((uintptr_t)base & 15) == 0, DLB_ERR_ALIGNMENT, "cache base is not 16-byte aligned");
+  DLB_CHECK_ARG((stride_page * 2) % 16 == 0 && (stride_slot * 2) % 16 == 0 && (stride_head * 2) % 16 == 0,
+                DLB_ERR_ALIGNMENT, "cache strides must be multiples of 16 bytes");
+  cuuint64_t dims[5] = {64, (cuuint64_t)heads, (cuuint64_t)slots, (cuuint64_t)(d / 64), (cuuint64_t)pages};
+  cuuint64_t strides[4] = {(cuuint64_t)stride_head * 2, (cuuint64_t)stride_slot * 2, 128, (cuuint64_t)stride_page * 2};
+  cuuint32_t box[5] = {64, 1, (cuuint32_t)box_slots, (cuuint32_t)(d / 64), 1};
+  cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+  CUresult r = enc(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<void*>(base), dims, strides, box, estr,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  DLB_CHECK_ARG(r == CUDA_SUCCESS, DLB_ERR_DRIVER, "cuTensorMapEncodeTiled(cache rows) failed with CUresult %d", (int)r);
+  return DLB_OK;
+}
+
+__device__ __forceinline__ void tma_load_5d(void* smem_dst, const CUtensorMap* tmap, uint64_t* bar, int c0, int c1, int c2,
+                                            int c3, int c4) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
+      ::"r"(smem_u32(smem_dst)),
+      "l"(tmap), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4)
+      : "memory");
+}
+
 __device__ __forceinline__ void tma_load_3d(void* smem_dst, const CUtensorMap* tmap, uint64_t* bar, int c0, int c1,
                                             int c2) {
   asm volatile(
@@ -45,6 +77,11 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
+__device__ __forceinline__ float min3(float a, float b, float c) {
+  float d;
+  asm("min.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 // Packed pairs of fp32 in one 64-bit register (sm_100 f32x2 arithmetic)
 __device__ __forceinline__ uint64_t pack_f2(float lo, float hi) {
   uint64_t r;
@@ -57,6 +94,11 @@ __device__ __forceinline__ void unpack_f2(uint64_t v, float& lo, float& hi) {
 __device__ __forceinline__ uint64_t fma_f2(uint64_t a, uint64_t b, uint64_t c) {
   uint64_t d;
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul_f2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
 __device__ __forceinline__ uint64_t add_f2(uint64_t a, uint64_t b) {

@@ -32,7 +32,6 @@ constexpr int CONSUMERS = 4;
 constexpr int THREADS = 32 * (CONSUMERS + 1);
 constexpr int STAGES = 2;
 constexpr int EDGE_ROWS = 16;
-constexpr int MAX_CLUSTER = 8;
 constexpr float RESCALE_THRESHOLD = 8.0f;                   // log2 units: P stays below 2^8, well inside fp16
 template <int D, int NH> struct Layout {
   static constexpr int HEADS = 8 * NH;                      // q-heads to a CTA
@@ -50,46 +49,11 @@ template <int D, int NH> struct Layout {
 };
 }  // namespace cd
 
-__device__ __forceinline__ void cluster_barrier() {
-  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
-}
-__device__ __forceinline__ uint32_t peer_address(uint32_t smem_addr, int rank) {
-  uint32_t at;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_addr), "r"(rank));
-  return at;
-}
-__device__ __forceinline__ float peer_load(uint32_t at) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
-  return v;
-}
-__device__ __forceinline__ float4 peer_load4(uint32_t at) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
-  return v;
-}
 __device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
   uint32_t r;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
-
-// One running result (m, l, four columns) takes in another.
-struct Joined {
-  float m = -INFINITY, l = 0.f;
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  __device__ __forceinline__ void add(float pm, float pl, const float4& po) {
-    if (pm == -CUDART_INF_F) return;                        // a piece without keys
-    const float top = fmaxf(m, pm);
-    const float a = m == -CUDART_INF_F ? 0.f : fast_exp2(m - top), b = fast_exp2(pm - top);
-    m = top;
-    l = l * a + pl * b;
-    o.x = o.x * a + po.x * b;
-    o.y = o.y * a + po.y * b;
-    o.z = o.z * a + po.z * b;
-    o.w = o.w * a + po.w * b;
-  }
-};
 
 template <typename T, int D, int NH, bool CAP, bool PREFIX>
 __global__ void __launch_bounds__(cd::THREADS, NH == 1 ? 3 : 2)
@@ -176,29 +140,35 @@ cluster_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
       tma_prefetch_desc(&edge_k);
       tma_prefetch_desc(&edge_v);
     }
-    // One table entry per lane: `units` pages (or pieces of 64 slots) to a tile, 32 / units tiles to a batch, the next
-    // batch under way while this one is used.
+    // One table entry per lane: `units` pages (or pieces of 64 slots) to a tile, 32 / units tiles to a batch.  The next batch's
+    // entries are asked for when this one's come into use, and looked at only then.
     const int unit_shift = min(p.page_shift, 6);
     const int units = TILE >> unit_shift, batch_tiles = 32 / units;
-    auto look_up = [&](int t) {
+    auto lane_token = [&](int t, bool& wanted) {             // first key of this lane's piece of the batch from tile t on
       t += lane / units;
-      if (t >= t_hi) return 0;
       int at, from, to;
       tile_keys(t, at, from, to);
       const int tok = at + ((lane % units) << unit_shift);
-      if (tok >= to || tok + (1 << unit_shift) <= from) return 0;          // nothing visible here: not looked at
-      const int column = tok >> p.page_shift;
-      const int page = load_index(p.block_table, (int64_t)b * p.bt_stride + column, p.table_is_int64);
-      if (page >= 0 && page < p.num_pages) return page;
-      if (kvh == 0 && hblk == 0) report_bad_page(p.status, b, column, page);
-      return 0;
+      wanted = t < t_hi && tok < to && tok + (1 << unit_shift) > from;     // else nothing visible here: not looked at
+      return tok;
     };
-    int pages = look_up(t_lo), pages_next = look_up(t_lo + batch_tiles);
+    auto entry = [&](int t) {
+      bool wanted;
+      const int64_t column = lane_token(t, wanted) >> p.page_shift;
+      return wanted ? load_index(p.block_table, (int64_t)b * p.bt_stride + column, p.table_is_int64) : 0;
+    };
+    int pages = 0, pages_next = entry(t_lo);
     for (int t = t_lo; t < t_hi; ++t) {
       const int i = t - t_lo, in_batch = i % batch_tiles;
-      if (i > 0 && in_batch == 0) {
+      if (in_batch == 0) {
         pages = pages_next;
-        pages_next = look_up(t + batch_tiles);
+        pages_next = entry(t + batch_tiles);
+        if (pages < 0 || pages >= p.num_pages) {
+          bool wanted;
+          const int column = lane_token(t, wanted) >> p.page_shift;
+          if (kvh == 0 && hblk == 0) report_bad_page(p.status, b, column, pages);
+          pages = 0;
+        }
       }
       const int s = i % STAGES;
       const uint32_t ph = (i / STAGES) & 1;
@@ -265,7 +235,7 @@ cluster_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
       if (lane == 0) *ext_splits = n;
     }
     const float scale2 = p.sm_scale * 1.4426950408889634f;
-    const float cap_in = CAP ? p.sm_scale / p.softcap : 0.f, cap_out = p.softcap * 1.4426950408889634f;
+    const float cap_in = CAP ? 2.f * 1.4426950408889634f * p.sm_scale / p.softcap : 0.f, cap_out = p.softcap * 1.4426950408889634f;
     const int mat = lane >> 3;      // ldmatrix: which 8x8 matrix this lane addresses
     const int mrow = lane & 7;
 
@@ -318,7 +288,7 @@ cluster_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           float v = sacc[n][u];
-          if (CAP) v = cap_out * tanhf(v * cap_in);
+          if (CAP) v = soft_cap(v, cap_in, cap_out);
           else v *= scale2;
           if (partly) {
             const int key = key0 + (lane >> 2) + (u >> 1) * 8;
@@ -417,12 +387,6 @@ cluster_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
   }
   __syncthreads();
   T* out = reinterpret_cast<T*>(p.out) + row * p.o_st;
-  auto store = [&](int r, int d, const Joined& j) {
-    if (d >= p.dv) return;
-    const float inv = j.l > 0.f ? 1.f / j.l : 0.f;
-    typename Elem<T>::T2 v[2] = {Elem<T>::from_f2(j.o.x * inv, j.o.y * inv), Elem<T>::from_f2(j.o.z * inv, j.o.w * inv)};
-    *reinterpret_cast<uint2*>(out + (int64_t)(head0 + r) * p.o_sh + d) = *reinterpret_cast<const uint2*>(v);
-  };
   for (int idx = threadIdx.x; idx < rows_valid * QUADS; idx += THREADS) {
     const int r = idx / QUADS, d = idx % QUADS * 4;
     Joined j;
@@ -430,7 +394,7 @@ cluster_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
     for (int w = 0; w < CONSUMERS; ++w)
       j.add(red_m[w * H + r], red_l[w * H + r], *reinterpret_cast<const float4*>(red_o + (w * H + r) * PITCH + d));
     if (!PREFIX && cluster == 1) {
-      store(r, d, j);
+      store_joined<T>(out + (int64_t)(head0 + r) * p.o_sh, d, p.dv, j);
     } else {
       *reinterpret_cast<float4*>(red_o + (CONSUMERS * H + r) * PITCH + d) = j.o;
       if (d == 0) {
@@ -446,72 +410,86 @@ cluster_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
   else __syncthreads();
   const uint32_t at_o = smem_u32(red_o + CONSUMERS * H * PITCH), at_m = smem_u32(red_m + CONSUMERS * H),
                  at_l = smem_u32(red_l + CONSUMERS * H);
+  // the own tokens are through; the launch with the prefix's partial results may still have been under way
+  if (PREFIX) wait_for_previous();
   const int ext = PREFIX ? *ext_splits : 0;
-  const int per_rank = (rows_valid * QUADS + cluster - 1) / cluster;
-  const int idx_hi = min(rows_valid * QUADS, (rank + 1) * per_rank);
-  for (int idx = rank * per_rank + threadIdx.x; idx < idx_hi; idx += THREADS) {
-    const int r = idx / QUADS, d = idx % QUADS * 4;
+  // Eight lanes take eight quads of a row; where this CTA has few of them, two or four such groups of lanes share their
+  // pieces.  Four loads of a lane are under way together; the CTAs of the cluster share the quads.
+  constexpr int OCTS = QUADS / 8, GROUPS = 4 * (CONSUMERS + 1);
+  const int g_lo = rows_valid * OCTS * rank / cluster, g_hi = rows_valid * OCTS * (rank + 1) / cluster;
+  const int parts_shift = (g_hi - g_lo) * 4 <= GROUPS ? 2 : (g_hi - g_lo) * 2 <= GROUPS ? 1 : 0;
+  const int parts = 1 << parts_shift, part = (lane >> 3) & (parts - 1);
+  const int64_t rows_all = p.tokens * p.hq;
+  for (int g0 = g_lo; g0 < g_hi; g0 += GROUPS >> parts_shift) {
+    const int g = g0 + ((int)(threadIdx.x >> 3) >> parts_shift);
+    const int r = min(g, g_hi - 1) / OCTS, d = (g % OCTS * 8 + (lane & 7)) * 4;
     Joined j;
-    for (int c = 0; c < cluster; ++c)
-      j.add(peer_load(peer_address(at_m + r * 4, c)), peer_load(peer_address(at_l + r * 4, c)),
-            peer_load4(peer_address(at_o + (r * PITCH + d) * 4, c)));
+    for (int c0 = part; c0 < cluster; c0 += 4 * parts) {
+      float m[4], l[4];
+      float4 o[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int c = min(c0 + u * parts, cluster - 1);
+        m[u] = peer_load(peer_address(at_m + r * 4, c));
+        l[u] = peer_load(peer_address(at_l + r * 4, c));
+        o[u] = peer_load4(peer_address(at_o + (r * PITCH + d) * 4, c));
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (c0 + u * parts < cluster) j.add(m[u], l[u], o[u]);
+    }
     if constexpr (PREFIX) {
-      const int64_t prow = row * p.hq + head0 + r, rows_all = p.tokens * p.hq;
-      for (int s = 0; s < ext; s += 4) {
+      const int64_t prow = row * p.hq + head0 + r;
+      for (int s = part; s < ext; s += 4 * parts) {
         float2 ml[4];
         float4 o[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-          const int64_t k = min(s + u, ext - 1) * rows_all + prow;
+          const int64_t k = min(s + u * parts, ext - 1) * rows_all + prow;
           ml[u] = p.prefix.ml[k];
           o[u] = *reinterpret_cast<const float4*>(p.prefix.o + k * D + d);
         }
 #pragma unroll
         for (int u = 0; u < 4; ++u)
-          if (s + u < ext) j.add(ml[u].x, ml[u].y, o[u]);
+          if (s + u * parts < ext) j.add(ml[u].x, ml[u].y, o[u]);
       }
     }
-    store(r, d, j);
+    for (int o = 8; o < 8 * parts; o <<= 1)
+      j.add(__shfl_xor_sync(0xffffffffu, j.m, o), __shfl_xor_sync(0xffffffffu, j.l, o),
+            make_float4(__shfl_xor_sync(0xffffffffu, j.o.x, o), __shfl_xor_sync(0xffffffffu, j.o.y, o),
+                        __shfl_xor_sync(0xffffffffu, j.o.z, o), __shfl_xor_sync(0xffffffffu, j.o.w, o)));
+    if (part == 0 && g < g_hi) store_joined<T>(out + (int64_t)(head0 + r) * p.o_sh, d, p.dv, j);
   }
   if (cluster > 1) cluster_barrier();    // a CTA's shared memory stays until its peers have read it
 }
 
-// CTAs to a (sequence, kv head): doubled while the launch leaves SMs without work, down to two tiles a CTA, and up to four
-// waves of the CTAs that are resident while a CTA keeps eight tiles.
+// CTAs to a (sequence, kv head), by the shortest sum over the waves: in tenths of a microsecond a CTA takes 40 for everything but
+// its tiles, 25 more for a join, and for a tile 10 alone on its SM, 13 beside another CTA, 22 where three share the memory.
+// Measured with 1 / 2 / 4 / 8 (us, tiles of 64 keys x 128 columns, 17 and 65 of them):
+//    32 pairs 26.6 / 18.5 / 16.4 / 16.4        64 pairs 71.6 / 49.2 / 40.9 / 49.2       (65)
+//   128 pairs 32.7 / 26.7 / 34.8 / 41.0       128 pairs 79.8 / 63.5 / 69.7 / 75.8       (65)
+//   256 pairs 38.9 / 49.2 / 53.2 / 71.6       512 pairs 200.7 / 188.4 / 188.4 / 215.0   (65)
 static int pick_cluster(int64_t pairs, int64_t tiles, int resident) {
-  int c = 1;
-  const int64_t slots = resident * sm_count(current_device());
-  while (c < cd::MAX_CLUSTER && ((pairs * c < slots && tiles >= 4 * c) || (pairs * c < 4 * slots && tiles >= 16 * c))) c *= 2;
-  return c;
+  int best = 1;
+  int64_t best_cost = INT64_MAX;
+  for (int c = 1; c <= MAX_CLUSTER; c *= 2) {
+    const int64_t slots = cluster_slots(c) * resident / 2, ctas = pairs * c, waves = (ctas + slots - 1) / slots;
+    const int64_t sms = sm_count(current_device());
+    const int64_t tile = waves > 1 || ctas > 2 * sms ? 22 : ctas > sms ? 13 : 10;
+    const int64_t cost = waves * ((tiles + c - 1) / c * tile + 40 + (c > 1 ? 25 : 0));
+    if (cost < best_cost) {
+      best = c;
+      best_cost = cost;
+    }
+  }
+  return best;
 }
 
 template <typename T, int D, int NH, bool CAP, bool PREFIX>
 static int launch_cluster(const CUtensorMap (&maps)[4], const ClusterDecodeParams& p, int cluster, cudaStream_t stream) {
-  auto kern = cluster_decode_kernel<T, D, NH, CAP, PREFIX>;
-  constexpr int SMEM = cd::Layout<D, NH>::SMEM;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
-  if (e != cudaSuccess) {
-    set_last_error("cluster_decode: cannot raise dynamic shared memory: %s", cudaGetErrorString(e));
-    return (int)e;
-  }
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = cluster;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(cluster, p.hkv * ((p.group + 8 * NH - 1) / (8 * NH)), p.batch);
-  cfg.blockDim = dim3(cd::THREADS);
-  cfg.dynamicSmemBytes = SMEM;
-  cfg.stream = stream;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, kern, maps[0], maps[1], maps[2], maps[3], p);
-  if (e != cudaSuccess) {
-    set_last_error("cluster_decode: launch failed: %s", cudaGetErrorString(e));
-    (void)cudaGetLastError();
-    return (int)e;
-  }
-  return DLB_OK;
+  return launch_in_clusters("cluster_decode", cluster_decode_kernel<T, D, NH, CAP, PREFIX>,
+                            dim3(cluster, p.hkv * ((p.group + 8 * NH - 1) / (8 * NH)), p.batch), cd::THREADS,
+                            cd::Layout<D, NH>::SMEM, cluster, PREFIX, stream, maps[0], maps[1], maps[2], maps[3], p);
 }
 template <typename T, int D, int NH>
 static int launch_cluster(const CUtensorMap (&maps)[4], const ClusterDecodeParams& p, int cluster, cudaStream_t stream) {

@@ -1,8 +1,19 @@
 // Single-token attention split over a thread-block cluster (cluster_decode.cu), as its callers see it.
 #pragma once
+#include <math_constants.h>
+
 #include "attention.cuh"
 
 namespace dlb {
+
+constexpr int MAX_CLUSTER = 8;
+
+// CTAs of two to an SM that run at the same time in clusters of c: a cluster stays inside a GPC, so that larger ones leave
+// slots empty (296, 296, 284 and 264 on the B200 that was asked).
+static inline int64_t cluster_slots(int c) {
+  const int64_t all = 2 * sm_count(current_device());
+  return c <= 2 ? all : c == 4 ? all * 95 / 100 : all * 88 / 100;
+}
 
 // Partial results of the shared prefixes, one row per (token, q-head): unnormalised output, then the reference maximum
 // (base-2 domain) and the sum that go with it.
@@ -57,6 +68,105 @@ __device__ __forceinline__ void group_rows(const PrefixPartials& p, int64_t toke
   const int64_t a = max((int64_t)0, min(lo, tokens));
   start = (int)a;
   n = (int)max((int64_t)0, min(hi, tokens) - a);
+}
+
+// cap * tanh(x) in the base-2 domain from one exponential and one reciprocal: tanh(x) = 1 - 2 / (1 + e^2x).  Off by 2^-22 of
+// the cap, like a score of that size; `in` = 2 log2(e) sm_scale / cap, `out` = cap log2(e).
+__device__ __forceinline__ float soft_cap(float s, float in, float out) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + fast_exp2(s * in)));
+  return fmaf(-2.f * out, r, out);
+}
+// The same for |x| <= 1 without the special-function unit: tanh(x) = x P(x^2), P interpolated at the 7 Chebyshev nodes of
+// [0, 1], off by 1.2e-7 (2^-23) with 32-bit coefficients.  Two scores at a time: `x` = sm_scale / cap, `out` = sm_scale log2(e).
+__device__ __forceinline__ uint64_t soft_cap_small(uint64_t s, uint64_t x, uint64_t out) {
+  const uint64_t u1 = mul_f2(s, x), u = mul_f2(u1, u1);
+  auto both = [](float c) { return pack_f2(c, c); };
+  uint64_t p = both(0.00103803f);
+  p = fma_f2(p, u, both(-0.00619432f));
+  p = fma_f2(p, u, both(0.02027971f));
+  p = fma_f2(p, u, both(-0.05345165f));
+  p = fma_f2(p, u, both(0.13325076f));
+  p = fma_f2(p, u, both(-0.33332828f));
+  p = fma_f2(p, u, both(0.99999995f));
+  return mul_f2(mul_f2(s, out), p);
+}
+
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t peer_address(uint32_t smem_addr, int rank) {
+  uint32_t at;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_addr), "r"(rank));
+  return at;
+}
+__device__ __forceinline__ float peer_load(uint32_t at) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 peer_load4(uint32_t at) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
+  return v;
+}
+// One running result (m, l, four columns) takes in another.
+struct Joined {
+  float m = -INFINITY, l = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  __device__ __forceinline__ void add(float pm, float pl, const float4& po) {
+    if (pm == -CUDART_INF_F) return;                        // a piece without keys
+    const float top = fmaxf(m, pm);
+    const float a = m == -CUDART_INF_F ? 0.f : fast_exp2(m - top), b = fast_exp2(pm - top);
+    m = top;
+    l = l * a + pl * b;
+    o.x = o.x * a + po.x * b;
+    o.y = o.y * a + po.y * b;
+    o.z = o.z * a + po.z * b;
+    o.w = o.w * a + po.w * b;
+  }
+};
+
+// Columns d .. d + 3 of an output row of dv, rounded once; a row that saw no key is zero.
+template <typename T> __device__ __forceinline__ void store_joined(T* out_row, int d, int dv, const Joined& j) {
+  if (d >= dv) return;
+  const float inv = j.l > 0.f ? 1.f / j.l : 0.f;
+  typename Elem<T>::T2 v[2] = {Elem<T>::from_f2(j.o.x * inv, j.o.y * inv), Elem<T>::from_f2(j.o.z * inv, j.o.w * inv)};
+  *reinterpret_cast<uint2*>(out_row + d) = *reinterpret_cast<const uint2*>(v);
+}
+
+// A launch that says so may start once every CTA of the launch before it has begun and called let_next_start (or ended); it
+// sees that launch's results behind wait_for_previous.
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// Launch in clusters of `cluster` CTAs along x; `early` as above.
+template <typename... Params, typename... Args>
+static int launch_in_clusters(const char* what, void (*kern)(Params...), dim3 grid, int threads, int smem, int cluster,
+                              bool early, cudaStream_t stream, const Args&... args) {
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e == cudaSuccess) {
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = early ? 2 : 1;
+    e = cudaLaunchKernelEx(&cfg, kern, args...);
+  }
+  if (e != cudaSuccess) {
+    set_last_error("%s: launch failed: %s", what, cudaGetErrorString(e));
+    (void)cudaGetLastError();
+    return (int)e;
+  }
+  return DLB_OK;
 }
 
 // `width` is the tile width (64 or 128); key_bound the keys that one sequence can see at most.

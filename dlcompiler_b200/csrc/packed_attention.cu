@@ -33,20 +33,22 @@ constexpr int BN = 64;            // keys per block
 constexpr int THREADS = 192;      // warps 0-3 softmax (TMEM quadrant = warp id), warp 4 TMA, warp 5 MMA
 constexpr int WARP_TMA = 4;
 constexpr int WARP_MMA = 5;
-constexpr int Q_BOX = BM * 128;   // one 64-wide (128 B) column box of the Q tile
-constexpr int KV_BOX = BN * 128;  // one 64-wide column box of a K or V tile
-constexpr int KV_STAGES = 2;
-constexpr int TMEM_COLS = 256;    // S0 [0,64) S1 [64,128) O [128,128+D)
+constexpr int KV_BOX = BN * 128;  // one 64-wide (128 B) column box of a K or V block
+constexpr int TMEM_COLS = 256;    // S0 [0,64) S1 [64,128), P over the first half of its S; O [128,128+D)
 constexpr float RESCALE_THRESHOLD = 8.0f;   // log2 units: P stays below 2^8, well inside fp16
 enum { PREFILL, PREFIX };
-template <int D> struct Layout {
+// ROWS of Q in shared memory, 128 or 64; the half that 64 leave free is a third pair of K and V buffers
+template <int D, int ROWS> struct Layout {
   static constexpr int BOXES = D / 64;
-  static constexpr int KV_BYTES = BOXES * KV_BOX;
+  static constexpr int STAGES = ROWS == 64 ? 3 : 2;
+  static constexpr int Q_BOX = ROWS * 128;                    // one 64-wide column box of the Q tile
+  static constexpr int KV_BYTES = BOXES * KV_BOX;             // one K or V block
   static constexpr int OFF_Q = 0;
   static constexpr int OFF_K = OFF_Q + BOXES * Q_BOX;
-  static constexpr int OFF_V = OFF_K + KV_STAGES * KV_BYTES;
-  static constexpr int OFF_CTRL = OFF_V + KV_STAGES * KV_BYTES;
-  static constexpr int SMEM_BYTES = OFF_CTRL + 160;
+  static constexpr int OFF_V = OFF_K + STAGES * KV_BYTES;
+  static constexpr int OFF_CTRL = OFF_V + STAGES * KV_BYTES;
+  static constexpr int SMEM_BYTES = OFF_CTRL + 192;
+  static_assert(OFF_V - OFF_Q >= ROWS * D * 4, "the join keeps O in 32 bits over Q and K");
 };
 }  // namespace pa
 
@@ -62,7 +64,9 @@ struct PackedParams {
   int hq, hkv, group, tile_tokens;
   uint32_t group_inv;             // ceil(2^16 / group): r / group = r * group_inv >> 16 for r < 128
   int tiles;                      // row tiles in the grid
+  int cluster;                    // CTAs that share a tile's keys, a power of two
   int page_shift, max_pages, num_pages, dv;
+  int k_whole, v_whole;           // a load fetches all columns of its rows (make_tmap_rows)
   int table_is_int64, start_is_int64, qlens_is_int64, lens_is_int64;
   int window, sinks;              // PREFILL
   float scale_log2, sm_scale, softcap;
@@ -116,19 +120,20 @@ __device__ __forceinline__ bool packed_tile(const PackedParams& p, int x, int& s
   return false;
 }
 
-template <typename T, int D, int MODE, bool CAP>
+template <typename T, int D, int MODE, int ROWS, bool CAP>
 __global__ void __launch_bounds__(pa::THREADS, 2)
 packed_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
                         const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ PackedParams p) {
   using namespace pa;
-  using L = Layout<D>;
-  constexpr int BOXES = L::BOXES, KV_BYTES = L::KV_BYTES;
+  using L = Layout<D, ROWS>;
+  constexpr int BOXES = L::BOXES, KV_BYTES = L::KV_BYTES, Q_BOX = L::Q_BOX, STAGES = L::STAGES;
   constexpr int OFF_Q = L::OFF_Q, OFF_K = L::OFF_K, OFF_V = L::OFF_V, OFF_CTRL = L::OFF_CTRL;
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   // ---- which tile: PREFILL has the kv heads of a tile side by side, PREFIX the row tiles of a (kv head, split), which
-  // read the same keys ----
-  int x = (int)blockIdx.x, kvh, split = 0;
+  // read the same keys; the CTAs of a cluster share one ----
+  const int cluster = p.cluster, rank = (int)blockIdx.x & (cluster - 1);
+  int x = (int)blockIdx.x / cluster, kvh, split = 0;
   if (MODE == PREFILL) {
     kvh = x % p.hkv;
     x /= p.hkv;
@@ -138,6 +143,7 @@ packed_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
     split = kvh / p.hkv;
     kvh -= split * p.hkv;
   }
+  if (MODE == PREFIX) let_next_start();
   int seq, tile, start, n, kv_len;
   if (!packed_tile<MODE>(p, x, seq, tile, start, n, kv_len)) return;
   const int q0 = tile * p.tile_tokens;
@@ -159,8 +165,12 @@ packed_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
     first_block = split * (p.prefix.chunk / BN);
     nb = (min(p.prefix.chunk, keys - split * p.prefix.chunk) + BN - 1) / BN;
   }
+  // this CTA's blocks
+  const int j_lo = nb * rank / cluster;
+  nb = nb * (rank + 1) / cluster - j_lo;
   // first key of the tile's block j
   auto block_key = [&](int j) {
+    j += j_lo;
     return (MODE == PREFILL ? (j < sink_blocks ? j : first_block + j - sink_blocks) : first_block + j) * BN;
   };
   // does some row of the tile see one of the keys [from, to)?
@@ -175,25 +185,26 @@ packed_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
       p.status[1] = 50;
     return;
   }
+  // block j uses the K and V buffers j % STAGES and waits for parity (j / STAGES) & 1 of their barriers; S and P have two buffers
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + OFF_CTRL);
   uint64_t* q_full = bars + 0;
-  uint64_t* k_full = bars + 1;     // [2]
-  uint64_t* v_full = bars + 3;     // [2]
-  uint64_t* s_full = bars + 5;     // [2] S_j done; K stage reusable
-  uint64_t* p_full = bars + 7;     // [2] P_j written
-  uint64_t* pv_done = bars + 9;    // [2] P_j V_j done; V stage reusable, O updated
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 11);
+  uint64_t* k_full = bars + 1;               // [STAGES]
+  uint64_t* v_full = k_full + STAGES;        // [STAGES]
+  uint64_t* qk_done = v_full + STAGES;       // [STAGES] S there; K buffer reusable
+  uint64_t* pv_done = qk_done + STAGES;      // [STAGES] O updated; V buffer reusable
+  uint64_t* p_full = pv_done + STAGES;       // [2] P written
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(p_full + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   if (warp == WARP_TMA && lane == 0) {
     mbar_init(q_full, 1);
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&k_full[i], 1);
-      mbar_init(&v_full[i], 1);
-      mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 128);
-      mbar_init(&pv_done[i], 1);
+    for (int h = 0; h < STAGES; ++h) {
+      mbar_init(&k_full[h], 1);
+      mbar_init(&v_full[h], 1);
+      mbar_init(&qk_done[h], 1);
+      mbar_init(&pv_done[h], 1);
     }
+    for (int h = 0; h < 2; ++h) mbar_init(&p_full[h], 128);
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -207,70 +218,84 @@ packed_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
   const uint32_t tmem_base = *tmem_slot;
   const uint32_t tmem_o = tmem_base + 128;
 
+  float m_ref = -CUDART_INF_F;                     // softmax warps: reference maximum (scaled, base-2 domain) and sum
+  float l_sum = 0.f;
+  const int row = threadIdx.x;                     // row of the tile == TMEM lane
+  const uint32_t lane_field = (uint32_t)(warp * 32) << 16;
+
   if (warp == WARP_TMA) {
     // ------------------------------ TMA producer ------------------------------
-    if (lane == 0 && nb > 0) {
-      tma_prefetch_desc(&tmap_q);
-      tma_prefetch_desc(&tmap_k);
-      tma_prefetch_desc(&tmap_v);
-      mbar_arrive_expect_tx(q_full, BOXES * p.group * p.tile_tokens * 128);
+    // Lane l fetches box l of a block: 64 / min(page, 64) boxes, one page each.  The table entries of 32 boxes are asked for at
+    // once, one per lane, and looked at when they come into use.  The loop is short on purpose: this warp shares its
+    // scheduler with two busy softmax warps, so an instruction takes it about ten clocks, and a late load holds up everything.
+    if (nb > 0) {
+      if (lane == 0) {
+        tma_prefetch_desc(&tmap_q);
+        tma_prefetch_desc(&tmap_k);
+        tma_prefetch_desc(&tmap_v);
+        mbar_arrive_expect_tx(q_full, BOXES * p.group * p.tile_tokens * 128);
 #pragma unroll
-      for (int bx = 0; bx < BOXES; ++bx)
-        tma_load_3d(smem + OFF_Q + bx * Q_BOX, &tmap_q, q_full, bx * 64, kvh * p.group, start + q0);
-      const int box_shift = min(p.page_shift, 6);
-      const int n_box = BN >> box_shift;
-      // Pages of a block, at most four; -1: no key of it is seen, nothing is fetched.  The look-up of block j + 1 runs
-      // behind the loads of block j, so that its latency is not between a freed stage and the next load.
-      int pg[4] = {-1, -1, -1, -1};
-      auto look_up = [&](int j) {
-        const int key0 = block_key(j);
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          if (u >= n_box) break;
-          const int tok = key0 + (u << box_shift);
-          pg[u] = -1;
-          if (!seen(tok, tok + (1 << box_shift))) continue;
-          const int column = tok >> p.page_shift;
-          int page = load_index(p.block_table, (int64_t)seq * p.bt_stride + column, p.table_is_int64);
-          if (page < 0 || page >= p.num_pages) {
-            report_bad_page(p.status, seq, column, page);
-            page = 0;
-          }
-          pg[u] = page;
-        }
+        for (int bx = 0; bx < BOXES; ++bx)
+          tma_load_3d(smem + OFF_Q + bx * Q_BOX, &tmap_q, q_full, bx * 64, kvh * p.group, start + q0);
+      }
+      const int box_shift = min(p.page_shift, 6), boxes_shift = 6 - box_shift, n_box = 1 << boxes_shift;
+      const int batch = 32 >> boxes_shift;                     // blocks to a batch of entries
+      const uint32_t box_bytes = (uint32_t)((128 * BOXES) << box_shift);
+      // first key of this lane's box of the batch from block j on; does some row see a key of it?
+      auto lane_key = [&](int j) { return block_key(j + (lane >> boxes_shift)) + ((lane & (n_box - 1)) << box_shift); };
+      auto wanted = [&](int j) {
+        return j + (lane >> boxes_shift) < nb && seen(lane_key(j), lane_key(j) + (1 << box_shift));
       };
-      auto load_block = [&](int j, int off, const CUtensorMap* tmap, uint64_t* full, const int (&page)[4]) {
-        uint8_t* dst = smem + off + (j & 1) * KV_BYTES;
-        const int key0 = block_key(j);
-        int boxes = 0;
-#pragma unroll
-        for (int u = 0; u < 4; ++u) boxes += u < n_box && page[u] >= 0 ? 1 : 0;
-        mbar_arrive_expect_tx(&full[j & 1], (uint32_t)((boxes << box_shift) * 128 * BOXES));
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          if (u >= n_box || page[u] < 0) continue;
-          const int slot = (key0 + (u << box_shift)) & ((1 << p.page_shift) - 1);
-#pragma unroll
-          for (int bx = 0; bx < BOXES; ++bx)
-            tma_load_4d(dst + bx * KV_BOX + (u << box_shift) * 128, tmap, &full[j & 1], bx * 64, kvh, slot, page[u]);
-        }
+      auto entry = [&](int j) {
+        return wanted(j) ? load_index(p.block_table, (int64_t)seq * p.bt_stride + (lane_key(j) >> p.page_shift), p.table_is_int64) : 0;
       };
-      look_up(0);
+      int pages = 0, pages_next = entry(0);
       for (int j = 0; j < nb; ++j) {
-        const int s = j & 1;
-        const uint32_t ph = (j >> 1) & 1;
-        int pv[4];
+        const int in_batch = j & (batch - 1);
+        if (in_batch == 0) {
+          pages = pages_next;
+          pages_next = entry(j + batch);
+          if (pages < 0 || pages >= p.num_pages) {
+            report_bad_page(p.status, seq, lane_key(j) >> p.page_shift, pages);
+            pages = 0;
+          }
+        }
+        const int s = j % STAGES;
+        const uint32_t ph = (j / STAGES) & 1;
+        const int key = block_key(j) + (lane << box_shift);
+        const bool fetch = lane < n_box && seen(key, key + (1 << box_shift));
+        const int page = __shfl_sync(0xffffffffu, pages, (in_batch << boxes_shift) + (lane & (n_box - 1)));
+        const int slot = key & ((1 << p.page_shift) - 1);
+        uint8_t* dst = smem + s * KV_BYTES + ((lane << box_shift) & (BN - 1)) * 128;
+        const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, fetch)) * box_bytes;
+        auto load = [&](uint8_t* to, const CUtensorMap* map, uint64_t* full, bool whole_rows) {
+          if (whole_rows) {
+            tma_load_5d(to, map, full, 0, kvh, slot, 0, page);
+          } else {
 #pragma unroll
-        for (int u = 0; u < 4; ++u) pv[u] = pg[u];
-        if (!mbar_wait(&s_full[s], ph ^ 1, abort_flag, p.status, 51, j)) break;
-        load_block(j, OFF_K, &tmap_k, k_full, pg);
-        if (j + 1 < nb) look_up(j + 1);
-        if (!mbar_wait(&pv_done[s], ph ^ 1, abort_flag, p.status, 52, j)) break;
-        load_block(j, OFF_V, &tmap_v, v_full, pv);
+            for (int bx = 0; bx < BOXES; ++bx) tma_load_4d(to + bx * KV_BOX, map, full, bx * 64, kvh, slot, page);
+          }
+        };
+        int ok = 1;
+        if (lane == 0) {
+          ok = mbar_wait(&qk_done[s], ph ^ 1, abort_flag, p.status, 51, j) ? 1 : 0;
+          if (ok) mbar_arrive_expect_tx(&k_full[s], bytes);
+        }
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+        if (!ok) break;
+        if (fetch) load(dst + OFF_K, &tmap_k, &k_full[s], p.k_whole);
+        if (lane == 0) {
+          ok = mbar_wait(&pv_done[s], ph ^ 1, abort_flag, p.status, 52, j) ? 1 : 0;
+          if (ok) mbar_arrive_expect_tx(&v_full[s], bytes);
+        }
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+        if (!ok) break;
+        if (fetch) load(dst + OFF_V, &tmap_v, &v_full[s], p.v_whole);
       }
     }
   } else if (warp == WARP_MMA) {
     // ------------------------------ MMA issuer ------------------------------
+    // One thread's MMAs run in the order of their issue, so S_{j+2} overwrites P_j only once P_j V_j has read it.
     if (lane == 0 && nb > 0) {
       bool ok = mbar_wait(q_full, 0, abort_flag, p.status, 53, 0);
       const uint64_t q_d0 = make_smem_desc(smem_u32(smem + OFF_Q), 16, 1024, 2);
@@ -281,173 +306,213 @@ packed_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
       const uint32_t v_lo0 = (uint32_t)v_d0, v_hi = (uint32_t)(v_d0 >> 32);
       for (int j = 0; ok && j <= nb; ++j) {
         if (j < nb) {
-          // S_j = Q K_j^T.  S buffer s also carried P_{j-2}: P_{j-2} V_{j-2} was issued before, and one thread's MMAs run in order
-          const int s = j & 1;
-          if (!mbar_wait(&k_full[s], (j >> 1) & 1, abort_flag, p.status, 54, j)) break;
+          // S_j = Q K_j^T
+          const int s = j % STAGES;
+          if (!mbar_wait(&k_full[s], (j / STAGES) & 1, abort_flag, p.status, 54, j)) break;
           tc_fence_after_sync();
           const uint32_t k_lo = k_lo0 + (uint32_t)s * (KV_BYTES >> 4);
 #pragma unroll
           for (int ks = 0; ks < D / 16; ++ks) {
             const uint32_t qoff = (uint32_t)(((ks >> 2) * Q_BOX + (ks & 3) * 32) >> 4);
             const uint32_t koff = (uint32_t)(((ks >> 2) * KV_BOX + (ks & 3) * 32) >> 4);
-            if (ks == 0) umma_ss_lohi<0>(tmem_base + s * BN, q_lo0 + qoff, kq_hi, k_lo + koff, kq_hi, p.idesc_qk);
-            else umma_ss_lohi<1>(tmem_base + s * BN, q_lo0 + qoff, kq_hi, k_lo + koff, kq_hi, p.idesc_qk);
+            if (ks == 0) umma_ss_lohi<0>(tmem_base + (j & 1) * BN, q_lo0 + qoff, kq_hi, k_lo + koff, kq_hi, p.idesc_qk);
+            else umma_ss_lohi<1>(tmem_base + (j & 1) * BN, q_lo0 + qoff, kq_hi, k_lo + koff, kq_hi, p.idesc_qk);
           }
-          umma_commit(&s_full[s]);
+          umma_commit(&qk_done[s]);
         }
         if (j > 0) {
           // O += P_{j-1} V_{j-1}
-          const int jj = j - 1, s = jj & 1;
-          const uint32_t ph = (jj >> 1) & 1;
-          const bool r1 = mbar_try_wait(&p_full[s], ph), r2 = mbar_try_wait(&v_full[s], ph);
+          const int jj = j - 1, s = jj % STAGES;
+          const uint32_t p_ph = (jj >> 1) & 1, v_ph = (jj / STAGES) & 1, pt = tmem_base + (jj & 1) * BN;
+          const bool r1 = mbar_try_wait(&p_full[jj & 1], p_ph), r2 = mbar_try_wait(&v_full[s], v_ph);
           if (!(r1 && r2)) {
-            if (!mbar_wait(&p_full[s], ph, abort_flag, p.status, 56, jj)) break;
-            if (!mbar_wait(&v_full[s], ph, abort_flag, p.status, 57, jj)) break;
+            if (!mbar_wait(&p_full[jj & 1], p_ph, abort_flag, p.status, 56, jj)) break;
+            if (!mbar_wait(&v_full[s], v_ph, abort_flag, p.status, 57, jj)) break;
           }
           tc_fence_after_sync();
           const uint32_t v_lo = v_lo0 + (uint32_t)s * (KV_BYTES >> 4);
-          if (jj == 0) umma_ts_lohi<0>(tmem_o, tmem_base + s * BN, v_lo, v_hi, p.idesc_pv);
-          else umma_ts_lohi<1>(tmem_o, tmem_base + s * BN, v_lo, v_hi, p.idesc_pv);
+          if (jj == 0) umma_ts_lohi<0>(tmem_o, pt, v_lo, v_hi, p.idesc_pv);
+          else umma_ts_lohi<1>(tmem_o, pt, v_lo, v_hi, p.idesc_pv);
 #pragma unroll
-          for (int ks = 1; ks < BN / 16; ++ks)
-            umma_ts_lohi<1>(tmem_o, tmem_base + s * BN + ks * 8, v_lo + ks * (16 * 128 >> 4), v_hi, p.idesc_pv);
+          for (int ks = 1; ks < BN / 16; ++ks) umma_ts_lohi<1>(tmem_o, pt + ks * 8, v_lo + ks * (16 * 128 >> 4), v_hi, p.idesc_pv);
           umma_commit(&pv_done[s]);
         }
       }
     }
   } else {
-    // ------------------------------ softmax / correction / epilogue ------------------------------
-    const int quad = warp;
-    const int row = quad * 32 + lane;              // row of the tile == TMEM lane
+    // ------------------------------ softmax / correction ------------------------------
     const bool live = row < tile_rows;
-    const int tok = (int)((uint32_t)row * p.group_inv >> 16);
-    const int q_pos = hist + q0 + tok;             // position of this row's token
-    const uint32_t lane_field = (uint32_t)(quad * 32) << 16;
-    float m_ref = -CUDART_INF_F;                   // reference maximum (scaled, base-2 domain)
-    float l_sum = 0.f;
+    const int q_pos = hist + q0 + (int)((uint32_t)row * p.group_inv >> 16);      // position of this row's token
+    const float cap_in = CAP ? 2.f * 1.4426950408889634f * p.sm_scale / p.softcap : 0.f, cap_out = p.softcap * 1.4426950408889634f,
+                cap_x = CAP ? p.sm_scale / p.softcap : 0.f;
+    const float eff_scale = CAP ? 1.f : p.scale_log2;
     bool ok = true;
+    // A warp whose rows are all past the tile's last one keeps in step and computes nothing: its P and O stay what they are, and
+    // no other row reads them.
+    const bool busy = warp * 32 < tile_rows;
     for (int j = 0; j < nb; ++j) {
-      const int s = j & 1;
-      const uint32_t ph = (j >> 1) & 1;
-      ok = mbar_wait(&s_full[s], ph, abort_flag, p.status, 58, j);
+      const int s = j % STAGES;
+      ok = mbar_wait(&qk_done[s], (j / STAGES) & 1, abort_flag, p.status, 58, j);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after_sync();
-      uint32_t sr[2][32];
-      tmem_ld_32x32b_x32(tmem_base + lane_field + s * BN, sr[0]);
-      tmem_ld_32x32b_x32(tmem_base + lane_field + s * BN + 32, sr[1]);
-      tmem_wait_ld();
-
-      float eff_scale = p.scale_log2;
-      if (CAP) {
-        const float inv = p.sm_scale / p.softcap, cap = p.softcap * 1.4426950408889634f;
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int c = 0; c < 32; ++c) sr[h][c] = __float_as_uint(cap * tanhf(__uint_as_float(sr[h][c]) * inv));
-        eff_scale = 1.f;
-      }
+      const uint32_t s_cols = tmem_base + lane_field + (j & 1) * BN;
       const int key0 = block_key(j);
-      // blocks that some row sees only in part: one bit per key of this row
+      // blocks that some row sees only in part
       const bool whole = MODE == PREFILL ? key0 + BN - 1 <= hist + q0 && key0 + BN <= keys && key0 >= pos_hi - p.window
                                          : key0 + BN <= keys;
-      if (!whole) {
-        const int hi = MODE == PREFILL ? min(q_pos, keys - 1) - key0 : keys - 1 - key0;      // last visible key
-        uint64_t bits = hi < 0 ? 0ull : hi >= BN - 1 ? ~0ull : (2ull << hi) - 1;
-        if (MODE == PREFILL) {
-          const int lo = q_pos - p.window - key0, sk = p.sinks - key0;
-          const uint64_t win = lo <= 0 ? ~0ull : lo >= BN ? 0ull : ~0ull << lo;
-          const uint64_t snk = sk <= 0 ? 0ull : sk >= BN ? ~0ull : (1ull << sk) - 1;
-          bits &= win | snk;
+      if (busy) {
+        uint32_t sr[2][32];
+        tmem_ld_32x32b_x32(s_cols, sr[0]);
+        tmem_ld_32x32b_x32(s_cols + 32, sr[1]);
+        tmem_wait_ld();
+        // largest score of the row, three at a time in four chains
+        auto largest = [&] {
+          float m4[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int c = 0; c < 32; c += 8) {
+#pragma unroll
+              for (int u = 0; u < 4; ++u)
+                m4[u] = max3(m4[u], __uint_as_float(sr[h][c + 2 * u]), __uint_as_float(sr[h][c + 2 * u + 1]));
+            }
+          }
+          return fmaxf(max3(m4[0], m4[1], m4[2]), m4[3]);
+        };
+        // one bit per key of this row that it sees
+        uint32_t word[2] = {~0u, ~0u};
+        if (!whole) {
+          const int hi = MODE == PREFILL ? min(q_pos, keys - 1) - key0 : keys - 1 - key0;      // last visible key
+          uint64_t bits = hi < 0 ? 0ull : hi >= BN - 1 ? ~0ull : (2ull << hi) - 1;
+          if (MODE == PREFILL) {
+            const int lo = q_pos - p.window - key0, sk = p.sinks - key0;
+            const uint64_t win = lo <= 0 ? ~0ull : lo >= BN ? 0ull : ~0ull << lo;
+            const uint64_t snk = sk <= 0 ? 0ull : sk >= BN ? ~0ull : (1ull << sk) - 1;
+            bits &= win | snk;
+          }
+          word[0] = (uint32_t)bits;
+          word[1] = (uint32_t)(bits >> 32);
         }
-        const uint32_t word[2] = {(uint32_t)bits, (uint32_t)(bits >> 32)};
+        auto hide = [&](uint32_t as) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+          for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int c = 0; c < 32; ++c)
-            if (!(word[h] >> c & 1u)) sr[h][c] = 0xff800000u;   // -inf
-      }
-      float mx4[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};   // 4 independent chains
+            for (int c = 0; c < 32; ++c)
+              if (!(word[h] >> c & 1u)) sr[h][c] = as;
+        };
+        float mx = 0.f;
+        if (CAP) {
+          // Scores below the cap, which they nearly always are, go through a polynomial: the exponential and the reciprocal of the
+          // other way take the special-function unit twice as long as the softmax itself.  Keys out of sight count as 0 so far:
+          // what was not fetched is anything.
+          if (!whole) hide(0u);
+          float m4[4] = {CUDART_INF_F, CUDART_INF_F, CUDART_INF_F, CUDART_INF_F};
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
+          for (int h = 0; h < 2; ++h) {
 #pragma unroll
-        for (int c = 0; c < 32; c += 8) {
+            for (int c = 0; c < 32; c += 8) {
 #pragma unroll
-          for (int u = 0; u < 4; ++u)
-            mx4[u] = max3(mx4[u], __uint_as_float(sr[h][c + 2 * u]), __uint_as_float(sr[h][c + 2 * u + 1]));
+              for (int u = 0; u < 4; ++u)
+                m4[u] = min3(m4[u], __uint_as_float(sr[h][c + 2 * u]), __uint_as_float(sr[h][c + 2 * u + 1]));
+            }
+          }
+          mx = largest();
+          const float size = fmaxf(mx, -fminf(min3(m4[0], m4[1], m4[2]), m4[3]));
+          if (!__any_sync(0xffffffffu, live && !(size * cap_x <= 1.f))) {
+            const uint64_t x2 = pack_f2(cap_x, cap_x), out2 = pack_f2(p.scale_log2, p.scale_log2);
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int c = 0; c < 32; c += 2) {
+                float a, b;
+                unpack_f2(soft_cap_small(pack_f2(__uint_as_float(sr[h][c]), __uint_as_float(sr[h][c + 1])), x2, out2), a, b);
+                sr[h][c] = __float_as_uint(a);
+                sr[h][c + 1] = __float_as_uint(b);
+              }
+          } else {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int c = 0; c < 32; ++c) sr[h][c] = __float_as_uint(soft_cap(__uint_as_float(sr[h][c]), cap_in, cap_out));
+          }
+          mx = soft_cap(mx, cap_in, cap_out);
         }
-      }
-      float mx = fmaxf(max3(mx4[0], mx4[1], mx4[2]), mx4[3]);
-      mx = live ? mx * eff_scale : -CUDART_INF_F;     // rows past the tile's last token never ask for a rescale
-      float alpha = 1.f;
-      bool rescale = false;
-      if (m_ref == -CUDART_INF_F) {
-        m_ref = mx;                                 // first visible block: nothing accumulated yet
-      } else if (mx - m_ref > RESCALE_THRESHOLD) {
-        alpha = fast_exp2(m_ref - mx);
-        m_ref = mx;
-        rescale = true;
-      }
-      // O may be rescaled only once P_{j-1} V_{j-1} has retired.  (P_{j-2} V_{j-2} retired before S_j was
-      // signalled, so the barrier is never more than one phase behind and the parity wait is exact.)
-      if (j > 0 && __any_sync(0xffffffffu, rescale)) {
-        ok = mbar_wait(&pv_done[(j - 1) & 1], ((j - 1) >> 1) & 1, abort_flag, p.status, 59, j);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        tc_fence_after_sync();
+        if (!whole) hide(0xff800000u);                // -inf
+        // p = 2^(s * scale - m) as 16-bit pairs, and their sum
+        uint32_t pk[2][16];
+        auto weigh = [&](float m) {
+          const uint64_t scale2 = pack_f2(eff_scale, eff_scale);
+          const float neg = m == -CUDART_INF_F ? 0.f : -m;
+          const uint64_t negm2 = pack_f2(neg, neg);
+          uint64_t sum2a = pack_f2(0.f, 0.f), sum2b = sum2a;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int c = 0; c < 32; c += 4) {
+              const uint64_t a01 = fma_f2(pack_f2(__uint_as_float(sr[h][c]), __uint_as_float(sr[h][c + 1])), scale2, negm2);
+              const uint64_t a23 = fma_f2(pack_f2(__uint_as_float(sr[h][c + 2]), __uint_as_float(sr[h][c + 3])), scale2, negm2);
+              float x0, x1, x2, x3;
+              unpack_f2(a01, x0, x1);
+              unpack_f2(a23, x2, x3);
+              const float e0 = fast_exp2(x0), e1 = fast_exp2(x1), e2 = fast_exp2(x2), e3 = fast_exp2(x3);
+              sum2a = add_f2(sum2a, pack_f2(e0, e1));
+              sum2b = add_f2(sum2b, pack_f2(e2, e3));
+              typename Elem<T>::T2 v01 = Elem<T>::from_f2(e0, e1);
+              typename Elem<T>::T2 v23 = Elem<T>::from_f2(e2, e3);
+              pk[h][c / 2] = *reinterpret_cast<uint32_t*>(&v01);
+              pk[h][c / 2 + 1] = *reinterpret_cast<uint32_t*>(&v23);
+            }
+          }
+          float a, b;
+          unpack_f2(add_f2(sum2a, sum2b), a, b);
+          return a + b;
+        };
+        // With the reference maximum as it is, which nearly always stays: so the exponentials do not wait for this block's maximum
+        float sum = weigh(m_ref);
+        if (!CAP || !whole) mx = largest() * eff_scale;
+        if (!live) mx = -CUDART_INF_F;                  // rows past the tile's last token never ask for more
+        // also a row's first visible key: m_ref is -inf until then (-inf - -inf is no number, and not above)
+        const bool raise = mx - m_ref > RESCALE_THRESHOLD;
+        if (__any_sync(0xffffffffu, raise)) {
+          const float alpha = raise ? fast_exp2(m_ref - mx) : 1.f;
+          if (raise) m_ref = mx;
+          if (j > 0) {
+            // O may be rescaled only once P_{j-1} V_{j-1} has retired (its barrier completes again only with a later block's P V,
+            // which waits for this one's P: the parity is exact).
+            ok = mbar_wait(&pv_done[(j - 1) % STAGES], ((j - 1) / STAGES) & 1, abort_flag, p.status, 59, j);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tc_fence_after_sync();
 #pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
-          uint32_t o[32];
-          tmem_ld_32x32b_x32(tmem_o + lane_field + c * 32, o);
-          tmem_wait_ld();
+            for (int c = 0; c < D / 32; ++c) {
+              uint32_t o[32];
+              tmem_ld_32x32b_x32(tmem_o + lane_field + c * 32, o);
+              tmem_wait_ld();
 #pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-          tmem_st_32x32b_x32(tmem_o + lane_field + c * 32, o);
+              for (int u = 0; u < 32; ++u) o[u] = __float_as_uint(__uint_as_float(o[u]) * alpha);
+              tmem_st_32x32b_x32(tmem_o + lane_field + c * 32, o);
+            }
+            tmem_wait_st();
+          }
+          l_sum *= alpha;
+          sum = weigh(m_ref);
         }
-        tmem_wait_st();
-      }
-      // p = 2^(s * scale - m), written back as 16-bit pairs over the first columns of the S buffer it came from
-      const float neg_m = (m_ref == -CUDART_INF_F) ? 0.f : -m_ref;
-      const uint64_t scale2 = pack_f2(eff_scale, eff_scale);
-      const uint64_t negm2 = pack_f2(neg_m, neg_m);
-      uint64_t sum2a = pack_f2(0.f, 0.f), sum2b = sum2a;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t pk[16];
-#pragma unroll
-        for (int c = 0; c < 32; c += 4) {
-          const uint64_t a01 =
-              fma_f2(pack_f2(__uint_as_float(sr[h][c]), __uint_as_float(sr[h][c + 1])), scale2, negm2);
-          const uint64_t a23 =
-              fma_f2(pack_f2(__uint_as_float(sr[h][c + 2]), __uint_as_float(sr[h][c + 3])), scale2, negm2);
-          float x0, x1, x2, x3;
-          unpack_f2(a01, x0, x1);
-          unpack_f2(a23, x2, x3);
-          const float e0 = fast_exp2(x0), e1 = fast_exp2(x1), e2 = fast_exp2(x2), e3 = fast_exp2(x3);
-          sum2a = add_f2(sum2a, pack_f2(e0, e1));
-          sum2b = add_f2(sum2b, pack_f2(e2, e3));
-          typename Elem<T>::T2 v01 = Elem<T>::from_f2(e0, e1);
-          typename Elem<T>::T2 v23 = Elem<T>::from_f2(e2, e3);
-          pk[c / 2] = *reinterpret_cast<uint32_t*>(&v01);
-          pk[c / 2 + 1] = *reinterpret_cast<uint32_t*>(&v23);
-        }
-        tmem_st_32x32b_x16(tmem_base + lane_field + s * BN + h * 16, pk);
-      }
-      {
-        float a, b;
-        unpack_f2(add_f2(sum2a, sum2b), a, b);
-        l_sum = l_sum * alpha + (a + b);
+        l_sum += sum;
+        // over the first columns of the block's S
+        tmem_st_32x32b_x16(s_cols, pk[0]);
+        tmem_st_32x32b_x16(s_cols + 16, pk[1]);
       }
       if (!whole && !(key0 >= vis_lo && key0 + BN <= vis_hi)) {
-        // V rows that no row of the tile sees (past the end, behind the window of every row, not fetched): their weights are
-        // zero, but 0 x (what a reused page or an old tile left there) may be NaN.  Zeroed, and made visible to the
+        // V rows that no row of the tile sees (past the end, behind the window of every row, not fetched): their weights
+        // are zero, but 0 x (what a reused page or an old tile left there) may be NaN.  Zeroed, and made visible to the
         // tensor core's reads, before this block's P V can be issued.
-        ok = mbar_wait(&v_full[s], ph, abort_flag, p.status, 61, j);
+        ok = mbar_wait(&v_full[s], (j / STAGES) & 1, abort_flag, p.status, 61, j);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         uint8_t* vt = smem + OFF_V + s * KV_BYTES;
-        for (int i = threadIdx.x; i < BN * BOXES * 8; i += 128) {
-          const int chunk = i & 7, bx = (i >> 3) % BOXES, r = (i >> 3) / BOXES;
+        for (int u = threadIdx.x; u < BN * BOXES * 8; u += 128) {
+          const int chunk = u & 7, bx = (u >> 3) % BOXES, r = (u >> 3) / BOXES;
           if (!seen(key0 + r, key0 + r + 1))
             *reinterpret_cast<uint4*>(vt + bx * KV_BOX + r * 128 + chunk * 16) = make_uint4(0u, 0u, 0u, 0u);
         }
@@ -455,68 +520,64 @@ packed_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
       }
       tmem_wait_st();
       tc_fence_before_sync();
-      mbar_arrive(&p_full[s]);
+      mbar_arrive(&p_full[j & 1]);
     }
     if (ok && nb > 0) {
-      ok = mbar_wait(&pv_done[(nb - 1) & 1], ((nb - 1) >> 1) & 1, abort_flag, p.status, 60, nb);
+      ok = mbar_wait(&pv_done[(nb - 1) % STAGES], ((nb - 1) / STAGES) & 1, abort_flag, p.status, 60, nb);
       ok = __all_sync(0xffffffffu, ok);
     }
-    if (ok) {
-      tc_fence_after_sync();
-      if constexpr (MODE == PREFIX) {
-        const int64_t rows_all = p.tokens * p.hq;
-        const int64_t at = split * rows_all + (int64_t)(start + q0 + tok) * p.hq + kvh * p.group + (row - tok * p.group);
-        float4* dst = reinterpret_cast<float4*>(p.prefix.o + at * D);
+    tc_fence_after_sync();
+    if (MODE == PREFIX || cluster > 1) {
+      // O in 32 bits over Q and K (every MMA has retired), 16-byte chunk q of row r at q ^ (r & 7); maximum and sum over V
+      float* ml = reinterpret_cast<float*>(smem + OFF_V);
+      ml[row] = ok ? m_ref : -CUDART_INF_F;
+      ml[BM + row] = l_sum;
 #pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
-          uint32_t o[32];
-          tmem_ld_32x32b_x32(tmem_o + lane_field + c * 32, o);
+      for (int c = 0; ok && busy && nb > 0 && c < D / 32; ++c) {
+        uint32_t o[32];
+        tmem_ld_32x32b_x32(tmem_o + lane_field + c * 32, o);
+        tmem_wait_ld();
+#pragma unroll
+        for (int v = 0; v < 8; ++v)
+          *reinterpret_cast<uint4*>(smem + OFF_Q + row * (D * 4) + (((c * 8 + v) ^ (row & 7)) << 4)) =
+              make_uint4(o[4 * v], o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]);
+      }
+    } else if (ok) {
+      // Through the Q tile's shared memory (every Q K^T has retired; row r of O over row r of Q, same swizzle), 64
+      // columns at a time, so that the lanes of a store cover whole 128-byte lines.  A row that saw no key is zero.
+      const float inv_l = l_sum > 0.f ? 1.f / l_sum : 0.f;
+      uint8_t* stage = smem + OFF_Q;
+      const int sub = lane >> 3, cc = lane & 7;              // row of four, 16-byte chunk of its line
+      T* obase = reinterpret_cast<T*>(p.out) + (int64_t)(start + q0) * p.o_st + (int64_t)kvh * p.group * p.o_sh + cc * 8;
+#pragma unroll 1
+      for (int c = 0; busy && c < D / 64; ++c) {
+        uint32_t o[2][32];
+        if (nb > 0) {
+          tmem_ld_32x32b_x32(tmem_o + lane_field + c * 64, o[0]);
+          tmem_ld_32x32b_x32(tmem_o + lane_field + c * 64 + 32, o[1]);
           tmem_wait_ld();
-          if (live) {
-#pragma unroll
-            for (int v = 0; v < 8; ++v)
-              dst[c * 8 + v] = make_float4(__uint_as_float(o[4 * v]), __uint_as_float(o[4 * v + 1]),
-                                           __uint_as_float(o[4 * v + 2]), __uint_as_float(o[4 * v + 3]));
-          }
         }
-        if (live) p.prefix.ml[at] = make_float2(m_ref, l_sum);
-      } else {
-        // Through the Q tile's shared memory (every Q K^T has retired; row r of O over row r of Q, same swizzle), 64
-        // columns at a time, so that the lanes of a store cover whole 128-byte lines.  A row that saw no key is zero.
-        const float inv_l = l_sum > 0.f ? 1.f / l_sum : 0.f;
-        uint8_t* stage = smem + OFF_Q;
-        const int sub = lane >> 3, cc = lane & 7;              // row of four, 16-byte chunk of its line
-        T* obase = reinterpret_cast<T*>(p.out) + (int64_t)(start + q0) * p.o_st + (int64_t)kvh * p.group * p.o_sh + cc * 8;
-#pragma unroll 1
-        for (int c = 0; quad * 32 < tile_rows && c < D / 64; ++c) {
-          uint32_t o[2][32];
-          if (nb > 0) {
-            tmem_ld_32x32b_x32(tmem_o + lane_field + c * 64, o[0]);
-            tmem_ld_32x32b_x32(tmem_o + lane_field + c * 64 + 32, o[1]);
-            tmem_wait_ld();
+#pragma unroll
+        for (int v = 0; v < 8; ++v) {
+          uint32_t w[4];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const int e = (v & 3) * 8 + 2 * u;
+            typename Elem<T>::T2 v2 = Elem<T>::from_f2(__uint_as_float(o[v >> 2][e]) * inv_l, __uint_as_float(o[v >> 2][e + 1]) * inv_l);
+            w[u] = l_sum > 0.f ? *reinterpret_cast<uint32_t*>(&v2) : 0u;
           }
+          *reinterpret_cast<uint4*>(stage + c * Q_BOX + row * 128 + ((v ^ (row & 7)) << 4)) =
+              make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        __syncwarp();
+        if (c * 64 + cc * 8 < p.dv) {
 #pragma unroll
-          for (int v = 0; v < 8; ++v) {
-            uint32_t w[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int e = (v & 3) * 8 + 2 * i;
-              typename Elem<T>::T2 v2 = Elem<T>::from_f2(__uint_as_float(o[v >> 2][e]) * inv_l, __uint_as_float(o[v >> 2][e + 1]) * inv_l);
-              w[i] = l_sum > 0.f ? *reinterpret_cast<uint32_t*>(&v2) : 0u;
-            }
-            *reinterpret_cast<uint4*>(stage + c * Q_BOX + row * 128 + ((v ^ (row & 7)) << 4)) =
-                make_uint4(w[0], w[1], w[2], w[3]);
-          }
-          __syncwarp();
-          if (c * 64 + cc * 8 < p.dv) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const int r = quad * 32 + i * 4 + sub;
-              if (r < tile_rows) {
-                const int t = (int)((uint32_t)r * p.group_inv >> 16);
-                *reinterpret_cast<uint4*>(obase + (int64_t)t * p.o_st + (int64_t)(r - t * p.group) * p.o_sh + c * 64) =
-                    *reinterpret_cast<const uint4*>(stage + c * Q_BOX + r * 128 + ((cc ^ (r & 7)) << 4));
-              }
+          for (int u = 0; u < 8; ++u) {
+            const int r = warp * 32 + u * 4 + sub;
+            if (r < tile_rows) {
+              const int t = (int)((uint32_t)r * p.group_inv >> 16);
+              *reinterpret_cast<uint4*>(obase + (int64_t)t * p.o_st + (int64_t)(r - t * p.group) * p.o_sh + c * 64) =
+                  *reinterpret_cast<const uint4*>(stage + c * Q_BOX + r * 128 + ((cc ^ (r & 7)) << 4));
             }
           }
         }
@@ -530,36 +591,68 @@ packed_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
     tc_fence_after_sync();
     tmem_dealloc(tmem_base, TMEM_COLS);
   }
+  if (MODE == PREFILL && cluster == 1) return;
+
+  // ------------------------------ join the cluster ------------------------------
+  // Each CTA takes its share of the rows from all of them, four columns at a time.
+  if (cluster > 1) cluster_barrier();
+  constexpr int QUADS = D / 4;
+  const uint32_t at_o = smem_u32(smem + OFF_Q), at_m = smem_u32(smem + OFF_V), at_l = at_m + BM * 4;
+  const int r_lo = tile_rows * rank / cluster, r_hi = tile_rows * (rank + 1) / cluster;
+  for (int idx = threadIdx.x; idx < (r_hi - r_lo) * QUADS; idx += THREADS) {
+    const int r = r_lo + idx / QUADS, q = idx % QUADS;
+    Joined j;
+    for (int c0 = 0; c0 < cluster; c0 += 4) {      // four pieces under way together
+      float m[4], l[4];
+      float4 o[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int c = min(c0 + u, cluster - 1);
+        m[u] = peer_load(peer_address(at_m + r * 4, c));
+        l[u] = peer_load(peer_address(at_l + r * 4, c));
+        o[u] = peer_load4(peer_address(at_o + r * (D * 4) + ((q ^ (r & 7)) << 4), c));
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (c0 + u < cluster) j.add(m[u], l[u], o[u]);
+    }
+    const int t = (int)((uint32_t)r * p.group_inv >> 16);
+    const int64_t token = start + q0 + t, head = kvh * p.group + (r - t * p.group);
+    if constexpr (MODE == PREFIX) {
+      const int64_t at = (split * p.tokens + token) * p.hq + head;
+      *reinterpret_cast<float4*>(p.prefix.o + at * D + q * 4) = j.o;
+      if (q == 0) p.prefix.ml[at] = make_float2(j.m, j.l);
+    } else {
+      store_joined<T>(reinterpret_cast<T*>(p.out) + token * p.o_st + head * p.o_sh, q * 4, p.dv, j);
+    }
+  }
+  if (cluster > 1) cluster_barrier();    // a CTA's shared memory stays until its peers have read it
 }
 
-template <typename T, int D, int MODE, bool CAP>
+template <typename T, int D, int MODE, int ROWS, bool CAP>
 static int launch_packed_x(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const PackedParams& p,
                            unsigned grid, cudaStream_t stream) {
-  auto kern = packed_attention_kernel<T, D, MODE, CAP>;
-  constexpr int SMEM = pa::Layout<D>::SMEM_BYTES;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
-  if (e != cudaSuccess) {
-    set_last_error("packed_attention: smem attribute: %s", cudaGetErrorString(e));
-    return (int)e;
-  }
-  kern<<<grid, pa::THREADS, SMEM, stream>>>(tq, tk, tv, p);
-  DLB_CUDA_LAUNCH_CHECK();
-  return DLB_OK;
+  return launch_in_clusters("packed_attention", packed_attention_kernel<T, D, MODE, ROWS, CAP>, dim3(grid * p.cluster), pa::THREADS,
+                            pa::Layout<D, ROWS>::SMEM_BYTES, p.cluster, false, stream, tq, tk, tv, p);
+}
+template <typename T, int D, int MODE>
+static int launch_packed_x(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const PackedParams& p,
+                           unsigned grid, cudaStream_t s) {
+  const bool cap = p.softcap > 0.f;
+  if (p.tile_tokens * p.group <= 64)
+    return cap ? launch_packed_x<T, D, MODE, 64, true>(tq, tk, tv, p, grid, s)
+               : launch_packed_x<T, D, MODE, 64, false>(tq, tk, tv, p, grid, s);
+  return cap ? launch_packed_x<T, D, MODE, 128, true>(tq, tk, tv, p, grid, s)
+             : launch_packed_x<T, D, MODE, 128, false>(tq, tk, tv, p, grid, s);
 }
 template <int MODE>
 static int launch_packed(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const PackedParams& p, int D,
                          int dtype, unsigned grid, cudaStream_t s) {
-  const bool cap = p.softcap > 0.f;
-  if (dtype == DLB_DTYPE_BF16) {
-    if (D == 128) return cap ? launch_packed_x<__nv_bfloat16, 128, MODE, true>(tq, tk, tv, p, grid, s)
-                             : launch_packed_x<__nv_bfloat16, 128, MODE, false>(tq, tk, tv, p, grid, s);
-    return cap ? launch_packed_x<__nv_bfloat16, 64, MODE, true>(tq, tk, tv, p, grid, s)
-               : launch_packed_x<__nv_bfloat16, 64, MODE, false>(tq, tk, tv, p, grid, s);
-  }
-  if (D == 128) return cap ? launch_packed_x<__half, 128, MODE, true>(tq, tk, tv, p, grid, s)
-                           : launch_packed_x<__half, 128, MODE, false>(tq, tk, tv, p, grid, s);
-  return cap ? launch_packed_x<__half, 64, MODE, true>(tq, tk, tv, p, grid, s)
-             : launch_packed_x<__half, 64, MODE, false>(tq, tk, tv, p, grid, s);
+  if (dtype == DLB_DTYPE_BF16)
+    return D == 128 ? launch_packed_x<__nv_bfloat16, 128, MODE>(tq, tk, tv, p, grid, s)
+                    : launch_packed_x<__nv_bfloat16, 64, MODE>(tq, tk, tv, p, grid, s);
+  return D == 128 ? launch_packed_x<__half, 128, MODE>(tq, tk, tv, p, grid, s)
+                  : launch_packed_x<__half, 64, MODE>(tq, tk, tv, p, grid, s);
 }
 
 // What both entry points take: types, head sizes, cache layout.  Returns DLB_OK or an error; `width` is the tile width.
@@ -599,11 +692,29 @@ static int log2_of(int64_t v) {
   return s;
 }
 
-static void set_shape(PackedParams& p, int64_t hq, int64_t hkv, int width, float sm_scale, float softcap, int dtype) {
+// CTAs to a (row tile, kv head).  In microseconds a CTA takes about 4 for everything but its blocks, 2 more for a join, and for
+// a block 0.6 alone on its SM and 0.9 beside another; the shortest sum over the waves is taken.
+static int pick_packed_cluster(int64_t pairs, int64_t blocks) {
+  int best = 1;
+  int64_t best_cost = INT64_MAX;
+  for (int c = 1; c <= MAX_CLUSTER; c *= 2) {
+    const int64_t slots = cluster_slots(c), ctas = pairs * c;
+    const int64_t cost = (ctas + slots - 1) / slots * ((blocks + c - 1) / c * (2 * ctas <= slots ? 6 : 9) + 40 + (c > 1 ? 20 : 0));
+    if (cost < best_cost) {
+      best = c;
+      best_cost = cost;
+    }
+  }
+  return best;
+}
+
+// `tokens` is how many tokens of a sequence (or group) there are at most, or on average: where their rows fit half a tile, tiles
+// are half as high, which leaves room for a third K and V buffer.
+static void set_shape(PackedParams& p, int64_t tokens, int64_t hq, int64_t hkv, int width, float sm_scale, float softcap, int dtype) {
   p.hq = (int)hq;
   p.hkv = (int)hkv;
   p.group = (int)(hq / hkv);
-  p.tile_tokens = pa::BM / p.group;
+  p.tile_tokens = (tokens * p.group <= pa::BM / 2 ? pa::BM / 2 : pa::BM) / p.group;
   p.group_inv = (65536u + p.group - 1) / p.group;
   p.scale_log2 = sm_scale * 1.4426950408889634f;
   p.sm_scale = sm_scale;
@@ -653,7 +764,7 @@ extern "C" int dlb_sink_attention(const void* q, const void* k_cache, const void
                                  v_stride_slot, v_stride_head, width, bound, dtype, s);
   }
   PackedParams p = {};
-  set_shape(p, hq, hkv, width, sm_scale, softcap, dtype);
+  set_shape(p, max_q_len, hq, hkv, width, sm_scale, softcap, dtype);
   p.out = out; p.q_start = q_start_loc; p.q_lens = q_seq_len; p.kv_lens = kv_seq_len; p.block_table = block_table;
   p.o_st = o_stride_t; p.o_sh = o_stride_h; p.bt_stride = bt_stride;
   p.tokens = total_q_tokens;
@@ -662,15 +773,19 @@ extern "C" int dlb_sink_attention(const void* q, const void* k_cache, const void
   p.table_is_int64 = table_is_int64; p.start_is_int64 = start_is_int64; p.qlens_is_int64 = qlen_is_int64; p.lens_is_int64 = kvlen_is_int64;
   p.window = win; p.sinks = snk; p.status = status;
   const int64_t tiles = total_q_tokens / p.tile_tokens + batch;      // sequences end inside a tile at most once each
-  DLB_CHECK_ARG(tiles * hkv < (1LL << 31), DLB_ERR_TOO_LARGE, "sink_attention: grid too large");
+  DLB_CHECK_ARG(tiles * hkv * MAX_CLUSTER < (1LL << 31), DLB_ERR_TOO_LARGE, "sink_attention: grid too large");
   p.tiles = (int)tiles;
+  const int64_t seen = window + p.tile_tokens + sinks < max_pages * page_size ? window + p.tile_tokens + sinks : max_pages * page_size;
+  p.cluster = pick_packed_cluster(tiles * hkv, (seen + pa::BN - 1) / pa::BN);
   CUtensorMap tq, tk, tv;
   rc = make_tmap_tokens(&tq, q, head_dim, hq, total_q_tokens, q_stride_h, q_stride_t, p.tile_tokens, p.group);
   if (rc != DLB_OK) return rc;
   const int box = (int)(page_size < pa::BN ? page_size : pa::BN);
-  rc = make_tmap_cache(&tk, k_cache, head_dim, hkv, page_size, num_pages, k_stride_page, k_stride_slot, k_stride_head, box);
+  p.k_whole = box == pa::BN && head_dim == width;
+  rc = make_tmap_rows(&tk, k_cache, head_dim, hkv, page_size, num_pages, k_stride_page, k_stride_slot, k_stride_head, box, p.k_whole);
   if (rc != DLB_OK) return rc;
-  rc = make_tmap_cache(&tv, v_cache, head_dim_v, hkv, page_size, num_pages, v_stride_page, v_stride_slot, v_stride_head, box);
+  p.v_whole = box == pa::BN && head_dim_v == width;
+  rc = make_tmap_rows(&tv, v_cache, head_dim_v, hkv, page_size, num_pages, v_stride_page, v_stride_slot, v_stride_head, box, p.v_whole);
   if (rc != DLB_OK) return rc;
   return launch_packed<pa::PREFILL>(tq, tk, tv, p, width, dtype, (unsigned)(tiles * hkv), s);
 }
@@ -688,7 +803,7 @@ extern "C" int dlb_shared_prefix_attention(
     int64_t o_stride_h, int64_t k_stride_page, int64_t k_stride_slot, int64_t k_stride_head, int64_t v_stride_page,
     int64_t v_stride_slot, int64_t v_stride_head, int64_t pt_stride, int64_t bt_stride, int prefix_table_is_int64,
     int prefix_len_is_int64, int group_start_is_int64, int table_is_int64, int kvlen_is_int64, int64_t chunk,
-    float sm_scale, float softcap, int dtype, int32_t* status, void* stream) {
+    int64_t cluster, float sm_scale, float softcap, int dtype, int32_t* status, void* stream) {
   DLB_NVTX("dlb_shared_prefix_attention");
   using namespace dlb;
   int width = 0;
@@ -700,6 +815,8 @@ extern "C" int dlb_shared_prefix_attention(
                 DLB_ERR_TOO_LARGE, "shared_prefix_attention: number of groups or length of a table out of range");
   DLB_CHECK_ARG(chunk >= 64 && chunk % 64 == 0 && chunk < (1LL << 31), DLB_ERR_BAD_ARG,
                 "shared_prefix_attention: chunk %lld must be a multiple of 64", (long long)chunk);
+  DLB_CHECK_ARG(cluster == 1 || cluster == 2 || cluster == 4 || cluster == 8, DLB_ERR_BAD_ARG,
+                "shared_prefix_attention: cluster %lld must be 1, 2, 4 or 8", (long long)cluster);
   if (batch == 0) return DLB_OK;
   DLB_CHECK_ARG(q && k_cache && v_cache && out && prefix_table && prefix_len && group_start && block_table && kv_seq_len &&
                     partial,
@@ -710,7 +827,7 @@ extern "C" int dlb_shared_prefix_attention(
   const int64_t splits = (prefix_max_pages * page_size + chunk - 1) / chunk;
   cudaStream_t s = (cudaStream_t)stream;
   PackedParams p = {};
-  set_shape(p, hq, hkv, width, sm_scale, softcap, dtype);
+  set_shape(p, (batch + groups - 1) / groups, hq, hkv, width, sm_scale, softcap, dtype);
   p.block_table = prefix_table; p.bt_stride = pt_stride; p.table_is_int64 = prefix_table_is_int64;
   p.tokens = batch;
   p.batch = (int)groups;
@@ -723,15 +840,18 @@ extern "C" int dlb_shared_prefix_attention(
   x.groups = (int)groups; x.lens_is_int64 = prefix_len_is_int64; x.start_is_int64 = group_start_is_int64;
   x.max_len = (int)(prefix_max_pages * page_size); x.chunk = (int)chunk;
   const int64_t tiles = batch / p.tile_tokens + (groups < batch ? groups : batch);
-  DLB_CHECK_ARG(tiles * hkv * splits < (1LL << 31), DLB_ERR_TOO_LARGE, "shared_prefix_attention: grid too large");
+  p.cluster = (int)cluster;
+  DLB_CHECK_ARG(tiles * hkv * splits * cluster < (1LL << 31), DLB_ERR_TOO_LARGE, "shared_prefix_attention: grid too large");
   p.tiles = (int)tiles;
   CUtensorMap tq, tk, tv;
   rc = make_tmap_tokens(&tq, q, head_dim, hq, batch, q_stride_h, q_stride_t, p.tile_tokens, p.group);
   if (rc != DLB_OK) return rc;
   const int box = (int)(page_size < pa::BN ? page_size : pa::BN);
-  rc = make_tmap_cache(&tk, k_cache, head_dim, hkv, page_size, num_pages, k_stride_page, k_stride_slot, k_stride_head, box);
+  p.k_whole = box == pa::BN && head_dim == width;
+  rc = make_tmap_rows(&tk, k_cache, head_dim, hkv, page_size, num_pages, k_stride_page, k_stride_slot, k_stride_head, box, p.k_whole);
   if (rc != DLB_OK) return rc;
-  rc = make_tmap_cache(&tv, v_cache, head_dim_v, hkv, page_size, num_pages, v_stride_page, v_stride_slot, v_stride_head, box);
+  p.v_whole = box == pa::BN && head_dim_v == width;
+  rc = make_tmap_rows(&tv, v_cache, head_dim_v, hkv, page_size, num_pages, v_stride_page, v_stride_slot, v_stride_head, box, p.v_whole);
   if (rc != DLB_OK) return rc;
   rc = launch_packed<pa::PREFIX>(tq, tk, tv, p, width, dtype, (unsigned)(tiles * hkv * splits), s);
   if (rc != DLB_OK) return rc;

@@ -15,32 +15,36 @@ from .. import _lib
 
 
 @lru_cache(maxsize=64)
-def _axis_of_freq(sections: tuple, interleaved: bool):
+def _axis_of_freq(sections: tuple, interleaved: bool, axes: int, freqs: int):
     """Axis of every frequency as a host byte array."""
+    assert len(sections) == axes and all(n >= 0 for n in sections) and sum(sections) == freqs, \
+        "sections: one count per axis, together as many as frequencies"
     if interleaved:
-        order = sorted((i, a) for a, n in enumerate(sections) for i in range(n))
-        axes = [a for _, a in order]
+        order = [a for _, a in sorted((i, a) for a, n in enumerate(sections) for i in range(n))]
     else:
-        axes = [a for a, n in enumerate(sections) for _ in range(n)]
-    return (ctypes.c_uint8 * max(len(axes), 1))(*axes)
+        order = [a for a, n in enumerate(sections) for _ in range(n)]
+    return (ctypes.c_uint8 * max(freqs, 1))(*order)
 
 
 def _launch(q, k, q_out, k_out, positions, inv_freq, axes, inverse):
     tokens, hq, dim = q.shape
-    qs, ks, qos, kos = q.stride(), k.stride(), q_out.stride(), k_out.stride()
-    lib = _lib.load()
     dev = q.device
     with _lib.on_device(dev):
-        rc = lib.dlb_multi_axis_rotary(
+        rc = _lib.load().dlb_multi_axis_rotary(
             q.data_ptr(), k.data_ptr(), q_out.data_ptr(), k_out.data_ptr(), positions.data_ptr(),
-            int(positions.dtype == torch.int64), positions.stride(0), inv_freq.data_ptr(), axes, positions.size(0),
-            tokens, hq, k.size(1), dim, 2 * inv_freq.numel(), qs[0], qs[1], ks[0], ks[1], qos[0], qos[1], kos[0],
-            kos[1], int(inverse), _lib.dtype_code(q), _lib.stream_ptr(dev))
+            positions.dtype is torch.int64, positions.stride(0), inv_freq.data_ptr(), axes, positions.size(0), tokens, hq,
+            k.size(1), dim, 2 * inv_freq.numel(), *q.stride()[:2], *k.stride()[:2], *q_out.stride()[:2],
+            *k_out.stride()[:2], inverse, _lib.dtype_code(q), _lib.stream_ptr(dev))
     _lib.check(rc, "apply_multi_axis_rotary")
 
 
 def _dense(t):
     return t if t.stride(-1) == 1 or t.size(-1) == 1 else t.contiguous()
+
+
+def _check_output(out, x):
+    assert out.shape == x.shape and out.dtype is x.dtype and (out.stride(-1) == 1 or out.size(-1) == 1), \
+        "q_embed / k_embed must have their input's shape and dtype, the last dimension contiguous"
 
 
 class _MultiAxisRotary(torch.autograd.Function):
@@ -92,30 +96,28 @@ def apply_multi_axis_rotary(
     are for calls without one.  Returns (q_embed, k_embed).
     """
     dev = _lib.require_cuda(q, k, positions, inv_freq, q_embed, k_embed)
-    assert q.dim() == 3 and k.dim() == 3 and k.size(0) == q.size(0) and k.size(2) == q.size(2), \
-        "q and k are [tokens, heads, dim] with the same tokens and dim"
-    assert k.dtype == q.dtype, "q and k must have one dtype"
-    assert positions.dim() == 2 and positions.size(1) == q.size(0), "positions are [axes, tokens]"
-    assert positions.dtype in (torch.int32, torch.int64), "positions must be int32 or int64"
-    assert inv_freq.dim() == 1 and inv_freq.dtype == torch.float32, "inv_freq is a vector of fp32"
+    assert q.dim() == 3 and k.dim() == 3 and positions.dim() == 2, "q and k are [tokens, heads, dim], positions [axes, tokens]"
+    (tokens, _, dim), (tokens_k, _, dim_k), (n_axes, places) = q.shape, k.shape, positions.shape
+    assert tokens_k == tokens and places == tokens and dim_k == dim, "q, k and positions need the same tokens, q and k the same dim"
+    assert k.dtype is q.dtype, "q and k must have one dtype"
+    assert positions.dtype is torch.int64 or positions.dtype is torch.int32, "positions must be int32 or int64"
+    assert inv_freq.dim() == 1 and inv_freq.dtype is torch.float32, "inv_freq is a vector of fp32"
     assert not inv_freq.requires_grad, "there is no gradient for inv_freq"
-    sections = tuple(int(n) for n in sections)
-    assert len(sections) == positions.size(0) and min(sections) >= 0 and sum(sections) == inv_freq.numel(), \
-        "sections: one count per axis, together as many as frequencies"
-    axes = _axis_of_freq(sections, bool(interleaved))
+    axes = _axis_of_freq(tuple(sections), bool(interleaved), n_axes, inv_freq.numel())
     if positions.stride(1) != 1:
         positions = positions.contiguous()
     inv_freq = inv_freq.contiguous()
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad):
+    if (q.requires_grad or k.requires_grad) and torch.is_grad_enabled():
         assert q_embed is None and k_embed is None, "outputs cannot be given where a gradient is wanted"
         return _MultiAxisRotary.apply(q, k, positions, inv_freq, axes, False)
     q, k = _dense(q), _dense(k)
     if q_embed is None:
-        q_embed = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        q_embed = torch.empty_like(q, memory_format=torch.contiguous_format)
+    else:
+        _check_output(q_embed, q)
     if k_embed is None:
-        k_embed = torch.empty(k.shape, dtype=k.dtype, device=dev)
-    for out, x in ((q_embed, q), (k_embed, k)):
-        assert out.shape == x.shape and out.dtype == x.dtype and (out.stride(-1) == 1 or out.size(-1) == 1), \
-            "q_embed / k_embed must have their input's shape and dtype, the last dimension contiguous"
+        k_embed = torch.empty_like(k, memory_format=torch.contiguous_format)
+    else:
+        _check_output(k_embed, k)
     _launch(q, k, q_embed, k_embed, positions, inv_freq, axes, False)
     return q_embed, k_embed

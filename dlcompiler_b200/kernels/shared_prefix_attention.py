@@ -10,24 +10,27 @@ import torch
 from torch import Tensor
 
 from .. import _lib
-from .sink_attention import _is64, check_paged
+from .sink_attention import check_paged, is64, rows_of_table
 
-_SLOTS = 148 * 2      # CTAs that are resident at a time
+# CTAs that run at a time, by the size of their clusters: a cluster stays inside a GPC, so that larger ones leave slots empty
+_SLOTS = {1: 296, 2: 296, 4: 280, 8: 256}
 
 
 @lru_cache(maxsize=256)
-def _pick_prefix_chunk(tiles: int, blocks: int) -> int:
-    """Tokens per split of the prefix: `tiles` (row tile, kv head) pairs, `blocks` blocks of 64 keys.  A CTA costs about six
-    blocks of set-up, output and joining, one of a pair on an SM about three halves of one alone; the split with
-    the shortest sum over the waves is taken."""
-    best, chunk = None, blocks
-    for splits in range(1, min(blocks, 128) + 1):
-        per = -(-blocks // splits)
-        ctas = tiles * -(-blocks // per)
-        cost = -(-ctas // _SLOTS) * (per + 6) * (2 if ctas <= _SLOTS // 2 else 3)
-        if best is None or cost < best:
-            best, chunk = cost, per
-    return chunk * 64
+def _pick_prefix_split(tiles: int, blocks: int):
+    """(tokens per split, CTAs per split) for `tiles` (row tile, kv head) pairs and `blocks` blocks of 64 keys.  In microseconds a
+    CTA takes about 0.7 for a block and 4 for the rest, a partial result 0.02 per pair (128 rows written and read again)
+    and 0.3 for its place in the join; the CTAs of a cluster join theirs among themselves in 1.  The shortest sum is taken."""
+    best, pick = None, (blocks, 1)
+    for cluster in (1, 2, 4, 8):
+        for splits in range(1, min(blocks, 64) + 1):
+            per = -(-blocks // splits)
+            splits = -(-blocks // per)
+            mine = -(-per // cluster)
+            cost = -(-tiles * splits * cluster // _SLOTS[cluster]) * (mine * 0.7 + 4 + (cluster > 1)) + splits * (0.02 * tiles + 0.3)
+            if best is None or cost < best:
+                best, pick = cost, (per, cluster)
+    return pick[0] * 64, pick[1]
 
 
 def shared_prefix_attention_fwd(
@@ -60,41 +63,28 @@ def shared_prefix_attention_fwd(
     and alignment as in `sink_attention_fwd`.
     """
     dev = _lib.require_cuda(q, k, v, o, prefix_offsets, prefix_seqlens, group_start, block_offsets, kv_seqlens)
-    q = check_paged(q, k, v, o)
-    batch, hq, dk = q.shape
-    pages, page, hkv, dv = v.shape
+    q, (batch, hq, hkv, dk, dv, page, pages), strides = check_paged(q, k, v, o)
     groups = prefix_seqlens.numel()
     assert groups >= 1 and group_start.numel() == groups + 1, "group_start: one more entry than prefixes"
-    assert prefix_offsets.dim() == 2 and prefix_offsets.size(0) >= groups and prefix_offsets.size(1) >= 1, \
-        "prefix_offsets: one row per prefix"
-    assert block_offsets.dim() == 2 and block_offsets.size(0) >= batch and block_offsets.size(1) >= 1, \
-        "block_offsets: one row per sequence"
+    prefix_offsets, prefix_pages, pt_stride = rows_of_table(prefix_offsets, groups, "prefix_offsets")
+    block_offsets, columns, bt_stride = rows_of_table(block_offsets, batch, "block_offsets")
     assert kv_seqlens.numel() >= batch, "kv_seqlens: one per sequence"
-    if prefix_offsets.stride(1) != 1:
-        prefix_offsets = prefix_offsets.contiguous()
-    if block_offsets.stride(1) != 1:
-        block_offsets = block_offsets.contiguous()
     prefix_seqlens, group_start, kv_seqlens = prefix_seqlens.contiguous(), group_start.contiguous(), kv_seqlens.contiguous()
-    if sm_scale is None:
-        sm_scale = dk ** -0.5
-    prefix_pages = prefix_offsets.size(1)
-    rows = 128 // (hq // hkv)             # tokens to a row tile
-    chunk = _pick_prefix_chunk((batch // rows + min(groups, batch)) * hkv, -(-prefix_pages * page // 64))
-    splits = -(-prefix_pages * page // chunk)
+    wide = (is64(prefix_offsets, "prefix_offsets"), is64(prefix_seqlens, "prefix_seqlens"), is64(group_start, "group_start"),
+            is64(block_offsets, "block_offsets"), is64(kv_seqlens, "kv_seqlens"))
+    most = prefix_pages * page
+    heads = hq // hkv
+    tokens = (64 if -(-batch // groups) * heads <= 64 else 128) // heads              # to a row tile
+    chunk, cluster = _pick_prefix_split((batch // tokens + min(groups, batch)) * hkv, -(-most // 64))
     lib = _lib.load()
-    floats = lib.dlb_shared_prefix_workspace_floats(batch, hq, max(dk, dv), splits)
-    partial = torch.empty(floats, dtype=torch.float32, device=dev)
-    status = _lib.status_word(dev)
-    (qs0, qs1, _), (os0, os1, _), (ks0, ks1, ks2, _), (vs0, vs1, vs2, _) = q.stride(), o.stride(), k.stride(), v.stride()
     with _lib.on_device(dev):
+        floats = lib.dlb_shared_prefix_workspace_floats(batch, hq, max(dk, dv), -(-most // chunk))
+        partial = torch.empty(floats, dtype=torch.float32, device=dev)
         rc = lib.dlb_shared_prefix_attention(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), prefix_offsets.data_ptr(),
             prefix_seqlens.data_ptr(), group_start.data_ptr(), block_offsets.data_ptr(), kv_seqlens.data_ptr(),
-            partial.data_ptr(), batch, groups, hq, hkv, dk, dv, page, pages, prefix_pages, block_offsets.size(1),
-            qs0, qs1, os0, os1, ks0, ks1, ks2, vs0, vs1, vs2, prefix_offsets.stride(0), block_offsets.stride(0),
-            _is64(prefix_offsets, "prefix_offsets"), _is64(prefix_seqlens, "prefix_seqlens"),
-            _is64(group_start, "group_start"), _is64(block_offsets, "block_offsets"), _is64(kv_seqlens, "kv_seqlens"),
-            chunk, float(sm_scale), float(logit_softcapping or -1.0), _lib.dtype_code(q), status.data_ptr(),
-            _lib.stream_ptr(dev))
+            partial.data_ptr(), batch, groups, hq, hkv, dk, dv, page, pages, prefix_pages, columns, *strides, pt_stride,
+            bt_stride, *wide, chunk, cluster, dk ** -0.5 if sm_scale is None else sm_scale, logit_softcapping or -1.0,
+            _lib.dtype_code(q), _lib.status_word(dev).data_ptr(), _lib.stream_ptr(dev))
     _lib.check(rc, "shared_prefix_attention_fwd")
     return o

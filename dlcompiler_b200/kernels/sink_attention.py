@@ -9,24 +9,47 @@ from torch import Tensor
 from .. import _lib
 
 
-def _is64(t: Tensor, name: str) -> int:
-    assert t.dtype in (torch.int32, torch.int64), f"{name} must be int32 or int64, got {t.dtype}"
-    return int(t.dtype == torch.int64)
+_IS64 = {torch.int32: 0, torch.int64: 1}
+
+
+def is64(t: Tensor, name: str) -> int:
+    code = _IS64.get(t.dtype)
+    assert code is not None, f"{name} must be int32 or int64, got {t.dtype}"
+    return code
+
+
+def rows_of_table(table: Tensor, rows: int, name: str):
+    """A block table (copied where its rows are not contiguous), its columns and the stride of its rows."""
+    assert table.dim() == 2, f"{name} has two dimensions"
+    have, columns = table.shape
+    assert have >= rows and columns >= 1, f"{name}: one row of pages for each of {rows}, got {tuple(table.shape)}"
+    stride, step = table.stride()
+    if step != 1:
+        table = table.contiguous()
+        stride = columns
+    return table, columns, stride
 
 
 def check_paged(q: Tensor, k: Tensor, v: Tensor, o: Tensor):
-    """What the paged operators of this module and of shared_prefix_attention take; returns q with rows that the copy
-    engine can fetch."""
-    assert q.dim() == 3 and k.dim() == 4 and v.dim() == 4, "q is [tokens, Hq, D], the caches [pages, page_size, Hkv, D]"
-    assert q.dtype in (torch.float16, torch.bfloat16) and k.dtype == v.dtype == o.dtype == q.dtype, \
+    """What the paged operators of this module and of shared_prefix_attention take.  Returns q with rows that the copy engine
+    can fetch, the sizes (tokens, Hq, Hkv, D, Dv, page size, pages) and the strides of q, o, k and v in the order of the
+    C entries."""
+    assert q.dim() == 3 and k.dim() == 4 and v.dim() == 4 and o.dim() == 3, \
+        "q and o are [tokens, Hq, D], the caches [pages, page_size, Hkv, D]"
+    dtype = q.dtype
+    assert (dtype is torch.bfloat16 or dtype is torch.float16) and k.dtype is dtype and v.dtype is dtype and o.dtype is dtype, \
         "q, the caches and o must be fp16 or bf16, all the same"
-    assert k.size(3) == q.size(2) and v.shape[:3] == k.shape[:3], "the caches do not fit q or each other"
-    assert o.dim() == 3 and o.shape[:2] == q.shape[:2] and o.size(2) == v.size(3), "o must be [tokens, Hq, Dv]"
-    assert q.size(1) % k.size(2) == 0 and q.size(1) <= 128 * k.size(2), "Hq: a multiple of Hkv, at most 128 to one"
-    assert k.stride(3) == 1 and v.stride(3) == 1 and o.stride(2) == 1, "the last dimension must be contiguous"
-    if q.stride(2) != 1 or q.stride(0) % 8 or q.stride(1) % 8 or q.data_ptr() % 16:
+    (tokens, hq, dk), (pages, page, hkv, dim_k), (*like, dv) = q.shape, k.shape, v.shape
+    assert dim_k == dk and like == [pages, page, hkv], "the caches do not fit q or each other"
+    assert o.shape == (tokens, hq, dv), "o must be [tokens, Hq, Dv]"
+    assert hkv > 0 and hq % hkv == 0 and hq <= 128 * hkv, "Hq: a multiple of Hkv, at most 128 to one"
+    (q_st, q_sh, q_last), (o_st, o_sh, o_last) = q.stride(), o.stride()
+    (*k_strides, k_last), (*v_strides, v_last) = k.stride(), v.stride()
+    assert k_last == 1 and v_last == 1 and o_last == 1, "the last dimension must be contiguous"
+    if q_last != 1 or q_st % 8 or q_sh % 8 or q.data_ptr() % 16:
         q = q.clone(memory_format=torch.contiguous_format)
-    return q
+        q_st, q_sh = hq * dk, dk
+    return q, (tokens, hq, hkv, dk, dv, page, pages), (q_st, q_sh, o_st, o_sh, *k_strides, *v_strides)
 
 
 def sink_attention_fwd(
@@ -61,29 +84,20 @@ def sink_attention_fwd(
     in their rows.
     """
     dev = _lib.require_cuda(q, k, v, o, block_offsets, q_start_loc, q_seqlens, kv_seqlens)
-    q = check_paged(q, k, v, o)
+    q, (tokens, hq, hkv, dk, dv, page, pages), strides = check_paged(q, k, v, o)
     batch = q_seqlens.numel()
-    assert block_offsets.dim() == 2 and block_offsets.size(0) >= batch and block_offsets.size(1) >= 1, \
-        "block_offsets: one row per sequence"
+    block_offsets, columns, bt_stride = rows_of_table(block_offsets, batch, "block_offsets")
     assert q_start_loc.numel() >= batch and kv_seqlens.numel() >= batch, "q_start_loc and kv_seqlens: one per sequence"
     assert window_size >= 0 and num_sinks >= 0 and max_seqlen >= 0, "window_size, num_sinks and max_seqlen must not be negative"
-    if block_offsets.stride(1) != 1:
-        block_offsets = block_offsets.contiguous()
     q_start_loc, q_seqlens, kv_seqlens = q_start_loc.contiguous(), q_seqlens.contiguous(), kv_seqlens.contiguous()
-    tokens, hq, dk = q.shape
-    pages, page, hkv, dv = v.shape
-    if sm_scale is None:
-        sm_scale = dk ** -0.5
-    status = _lib.status_word(dev)
-    (qs0, qs1, _), (os0, os1, _), (ks0, ks1, ks2, _), (vs0, vs1, vs2, _) = q.stride(), o.stride(), k.stride(), v.stride()
+    wide = (is64(block_offsets, "block_offsets"), is64(q_start_loc, "q_start_loc"), is64(q_seqlens, "q_seqlens"),
+            is64(kv_seqlens, "kv_seqlens"))
     lib = _lib.load()
     with _lib.on_device(dev):
         rc = lib.dlb_sink_attention(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), block_offsets.data_ptr(), q_start_loc.data_ptr(),
             q_seqlens.data_ptr(), kv_seqlens.data_ptr(), batch, tokens, int(max_seqlen), hq, hkv, dk, dv, page, pages,
-            block_offsets.size(1), qs0, qs1, os0, os1, ks0, ks1, ks2, vs0, vs1, vs2, block_offsets.stride(0),
-            _is64(block_offsets, "block_offsets"), _is64(q_start_loc, "q_start_loc"), _is64(q_seqlens, "q_seqlens"),
-            _is64(kv_seqlens, "kv_seqlens"), int(window_size), int(num_sinks), float(sm_scale),
-            float(logit_softcapping or -1.0), _lib.dtype_code(q), status.data_ptr(), _lib.stream_ptr(dev))
+            columns, *strides, bt_stride, *wide, int(window_size), int(num_sinks), dk ** -0.5 if sm_scale is None else sm_scale,
+            logit_softcapping or -1.0, _lib.dtype_code(q), _lib.status_word(dev).data_ptr(), _lib.stream_ptr(dev))
     _lib.check(rc, "sink_attention_fwd")
     return o

@@ -312,7 +312,7 @@ int dlb_sink_attention(const void* q, const void* k_cache, const void* v_cache, 
  * prefix of its group, then its own tokens.  q [batch, hq, head_dim], out [batch, hq, head_dim_v]; group g is the
  * sequences group_start[g] .. group_start[g + 1] - 1 (group_start [groups + 1]), its prefix the first prefix_len[g] tokens
  * of row g of prefix_table [groups, prefix_max_pages]; a sequence's own tokens are the first kv_seq_len[b] of row b of
- * block_table [batch, max_pages].  `chunk` (a multiple of 64) tokens of a prefix go to a split; `partial` is a workspace
+ * block_table [batch, max_pages].  `chunk` (a multiple of 64) tokens of a prefix go to a split, which `cluster` (1, 2, 4 or 8) CTAs share; `partial` is a workspace
  * of dlb_shared_prefix_workspace_floats(batch, hq, larger head size, ceil(prefix_max_pages * page_size / chunk)) fp32,
  * 16-byte aligned, in use until the call's work on the stream is done.  Two launches.  Everything else as for
  * dlb_sink_attention.  No counterpart in the reference. */
@@ -327,7 +327,7 @@ int dlb_shared_prefix_attention(const void* q, const void* k_cache, const void* 
                                 int64_t v_stride_page, int64_t v_stride_slot, int64_t v_stride_head, int64_t pt_stride,
                                 int64_t bt_stride, int prefix_table_is_int64, int prefix_len_is_int64,
                                 int group_start_is_int64, int table_is_int64, int kvlen_is_int64, int64_t chunk,
-                                float sm_scale, float softcap, int dtype, int32_t* status, void* stream);
+                                int64_t cluster, float sm_scale, float softcap, int dtype, int32_t* status, void* stream);
 
 /* rms_norm with optional residual add.  new_x = x + residual in the storage dtype (written to
  * out_residual when given); out = w * (new_x * rsqrt(mean(new_x^2) + eps)).  weight_after_cast = 0

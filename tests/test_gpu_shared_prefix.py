@@ -204,3 +204,4 @@ def test_large_scores(cuda_device):
     b = Groups(cuda_device, [20], [700], list(range(20)), dtype=FP)
     b.q *= 12
     b.check(b.run())
+    b.check(b.run(cap=20.0), cap=20.0)                       # scores on both sides of the cap

@@ -120,6 +120,10 @@ SEVERAL = [  # new, past, window, sinks, page, hq, hkv, d, dv, dtype, cap
     ([40], [90], 17, 3, 16, 100, 1, 40, 48, BF, 15.0),
     ([7] * 40, [13 * i for i in range(40)], 100, 5, 16, 4, 2, 64, 64, BF, 0.0),
     ([1500], [0], 700, 4, 64, 8, 2, 128, 128, BF, 0.0),
+    ([5, 2, 9], [5000, 700, 0], 4095, 4, 16, 28, 4, 128, 128, FP, 0.0),
+    ([3], [2500], 1023, 70, 64, 4, 4, 64, 64, BF, 20.0),
+    ([2500, 1, 2400], [0, 30, 333], 300, 4, 64, 8, 8, 64, 64, BF, 0.0),
+    ([700, 19, 691], [1000, 0, 5], 200, 70, 16, 28, 4, 128, 128, FP, 25.0),
     ([3, 200], [50, 3], 5000, 10 ** 6, 64, 8, 2, 128, 128, BF, 0.0),
 ]
 
@@ -265,6 +269,7 @@ def test_large_scores_and_infinite_values_behind_the_window(cuda_device):
         flat_k, flat_v = b.k.view(-1, 2, 64), b.v.view(-1, 2, 64)
         flat_k[hidden], flat_v[hidden] = float("-inf"), torch.finfo(FP).min
         b.check(b.run())
+        b.check(b.run(cap=20.0), cap=20.0)                   # scores on both sides of the cap
 
 
 def test_empty_calls(cuda_device):

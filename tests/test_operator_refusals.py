@@ -133,27 +133,29 @@ def test_attention_entries():
     for nothing in (dict(batch=0), dict(tokens=0), dict(most=0)):
         assert sink(**nothing) == 0
 
-    def prefix(q=16, partial=16, batch=3, groups=2, hq=4, hkv=2, d=64, page=16, prefix_cols=2, cols=2, chunk=64,
+    def prefix(q=16, partial=16, batch=3, groups=2, hq=4, hkv=2, d=64, page=16, prefix_cols=2, cols=2, chunk=64, cluster=1,
                scale=0.1, dtype=_lib.DTYPE_BF16):
         return lib.dlb_shared_prefix_attention(q, 16, 16, 16, 16, 16, 16, 16, 16, partial, batch, groups, hq, hkv, d, 64,
                                                page, 4, prefix_cols, cols, 256, 64, 256, 64, 2048, 128, 64, 2048, 128, 64,
-                                               2, 2, 0, 0, 0, 0, 0, chunk, scale, -1.0, dtype, None, None)
+                                               2, 2, 0, 0, 0, 0, 0, chunk, cluster, scale, -1.0, dtype, None, None)
 
     for bad in (dict(q=None), dict(partial=None), dict(partial=8), dict(batch=-1), dict(groups=0), dict(groups=80000),
                 dict(hq=3), dict(d=12), dict(page=8), dict(prefix_cols=0), dict(cols=0), dict(chunk=0), dict(chunk=100),
+                dict(cluster=0), dict(cluster=3), dict(cluster=16),
                 dict(scale=0.0), dict(dtype=_lib.DTYPE_F32), dict(prefix_cols=1 << 28), dict(cols=1 << 28)):
         assert prefix(**bad) < 0 and lib.dlb_last_error().startswith(b"shared_prefix_attention"), bad
     assert prefix(batch=0) == 0
     assert lib.dlb_shared_prefix_workspace_floats(3, 4, 96, 5) == 3 * 4 * 5 * 130
 
 
-def test_prefix_chunk_rule():
-    """Chunks are whole blocks, cover the table, and leave no more splits than blocks."""
-    from dlcompiler_b200.kernels.shared_prefix_attention import _pick_prefix_chunk
+def test_prefix_split_rule():
+    """Chunks are whole blocks and no longer than the table; few rows are split over the SMs, many are not."""
+    from dlcompiler_b200.kernels.shared_prefix_attention import _pick_prefix_split
 
     for tiles in (1, 8, 64, 72, 296, 5000):
         for blocks in (1, 2, 16, 63, 512, 1876, 30000):
-            chunk = _pick_prefix_chunk(tiles, blocks)
-            assert chunk % 64 == 0 and 64 <= chunk <= blocks * 64
-    assert _pick_prefix_chunk(5000, 512) == 512 * 64          # enough rows: not split
-    assert _pick_prefix_chunk(8, 1876) < 1876 * 64 // 18      # few rows: split over the SMs
+            chunk, cluster = _pick_prefix_split(tiles, blocks)
+            assert chunk % 64 == 0 and 64 <= chunk <= blocks * 64 and cluster in (1, 2, 4, 8)
+    assert _pick_prefix_split(5000, 512) == (512 * 64, 1)
+    chunk, cluster = _pick_prefix_split(8, 1876)
+    assert 8 * cluster * -(-1876 * 64 // chunk) > 148
