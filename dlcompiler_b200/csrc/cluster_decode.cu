@@ -487,9 +487,9 @@ static int pick_cluster(int64_t pairs, int64_t tiles, int resident) {
 
 template <typename T, int D, int NH, bool CAP, bool PREFIX>
 static int launch_cluster(const CUtensorMap (&maps)[4], const ClusterDecodeParams& p, int cluster, cudaStream_t stream) {
-  return launch_in_clusters("cluster_decode", cluster_decode_kernel<T, D, NH, CAP, PREFIX>,
-                            dim3(cluster, p.hkv * ((p.group + 8 * NH - 1) / (8 * NH)), p.batch), cd::THREADS,
-                            cd::Layout<D, NH>::SMEM, cluster, PREFIX, stream, maps[0], maps[1], maps[2], maps[3], p);
+  return launch_in_clusters<cluster_decode_kernel<T, D, NH, CAP, PREFIX>>(
+      "cluster_decode", dim3(cluster, p.hkv * ((p.group + 8 * NH - 1) / (8 * NH)), p.batch), cd::THREADS,
+      cd::Layout<D, NH>::SMEM, cluster, PREFIX, stream, maps[0], maps[1], maps[2], maps[3], p);
 }
 template <typename T, int D, int NH>
 static int launch_cluster(const CUtensorMap (&maps)[4], const ClusterDecodeParams& p, int cluster, cudaStream_t stream) {

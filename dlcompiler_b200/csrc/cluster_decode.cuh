@@ -2,6 +2,8 @@
 #pragma once
 #include <math_constants.h>
 
+#include <atomic>
+
 #include "attention.cuh"
 
 namespace dlb {
@@ -77,18 +79,17 @@ __device__ __forceinline__ float soft_cap(float s, float in, float out) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + fast_exp2(s * in)));
   return fmaf(-2.f * out, r, out);
 }
-// The same for |x| <= 1 without the special-function unit: tanh(x) = x P(x^2), P interpolated at the 7 Chebyshev nodes of
-// [0, 1], off by 1.2e-7 (2^-23) with 32-bit coefficients.  Two scores at a time: `x` = sm_scale / cap, `out` = sm_scale log2(e).
-__device__ __forceinline__ uint64_t soft_cap_small(uint64_t s, uint64_t x, uint64_t out) {
+// The same for |x| <= 1 (TERMS = 7) or 1/4 (3) without the special-function unit: tanh(x) = x P(x^2), P interpolated at the
+// Chebyshev nodes of [0, 1] or [0, 1/16], off by 1.2e-7 (2^-23) with 32-bit coefficients.  Two scores at a time:
+// `x` = sm_scale / cap, `out` = sm_scale log2(e).
+template <int TERMS> __device__ __forceinline__ uint64_t soft_cap_small(uint64_t s, uint64_t x, uint64_t out) {
+  constexpr float P7[7] = {0.99999995f, -0.33332828f, 0.13325076f, -0.05345165f, 0.02027971f, -0.00619432f, 0.00103803f};
+  constexpr float P3[3] = {0.99999958f, -0.33321896f, 0.12841433f};
   const uint64_t u1 = mul_f2(s, x), u = mul_f2(u1, u1);
-  auto both = [](float c) { return pack_f2(c, c); };
-  uint64_t p = both(0.00103803f);
-  p = fma_f2(p, u, both(-0.00619432f));
-  p = fma_f2(p, u, both(0.02027971f));
-  p = fma_f2(p, u, both(-0.05345165f));
-  p = fma_f2(p, u, both(0.13325076f));
-  p = fma_f2(p, u, both(-0.33332828f));
-  p = fma_f2(p, u, both(0.99999995f));
+  auto term = [](int i) { return TERMS == 7 ? pack_f2(P7[i], P7[i]) : pack_f2(P3[i % 3], P3[i % 3]); };
+  uint64_t p = term(TERMS - 1);
+#pragma unroll
+  for (int i = TERMS - 2; i >= 0; --i) p = fma_f2(p, u, term(i));
   return mul_f2(mul_f2(s, out), p);
 }
 
@@ -140,11 +141,17 @@ template <typename T> __device__ __forceinline__ void store_joined(T* out_row, i
 __device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
-// Launch in clusters of `cluster` CTAs along x; `early` as above.
-template <typename... Params, typename... Args>
-static int launch_in_clusters(const char* what, void (*kern)(Params...), dim3 grid, int threads, int smem, int cluster,
-                              bool early, cudaStream_t stream, const Args&... args) {
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+// Launch in clusters of `cluster` CTAs along x; `early` as above.  The kernel's shared memory is raised once per device.
+template <auto KERN, typename... Args>
+static int launch_in_clusters(const char* what, dim3 grid, int threads, int smem, int cluster, bool early,
+                              cudaStream_t stream, const Args&... args) {
+  static std::atomic<uint64_t> raised{0};
+  const int dev = current_device();
+  cudaError_t e = cudaSuccess;
+  if (dev >= 64 || !(raised.load(std::memory_order_relaxed) >> dev & 1)) {
+    e = cudaFuncSetAttribute(KERN, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e == cudaSuccess && dev < 64) raised.fetch_or(1ull << dev, std::memory_order_relaxed);
+  }
   if (e == cudaSuccess) {
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -159,7 +166,7 @@ static int launch_in_clusters(const char* what, void (*kern)(Params...), dim3 gr
     cfg.stream = stream;
     cfg.attrs = attr;
     cfg.numAttrs = early ? 2 : 1;
-    e = cudaLaunchKernelEx(&cfg, kern, args...);
+    e = cudaLaunchKernelEx(&cfg, KERN, args...);
   }
   if (e != cudaSuccess) {
     set_last_error("%s: launch failed: %s", what, cudaGetErrorString(e));

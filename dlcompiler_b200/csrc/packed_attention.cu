@@ -23,6 +23,8 @@
 // that hold no key which the tile sees.
 #include <math_constants.h>
 
+#include <type_traits>
+
 #include "cluster_decode.cuh"
 
 namespace dlb {
@@ -403,7 +405,7 @@ packed_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
         };
         float mx = 0.f;
         if (CAP) {
-          // Scores below the cap, which they nearly always are, go through a polynomial: the exponential and the reciprocal of the
+          // Scores below the cap, which they nearly always are, go through a polynomial, a short one below a quarter of it: the exponential and the reciprocal of the
           // other way take the special-function unit twice as long as the softmax itself.  Keys out of sight count as 0 so far:
           // what was not fetched is anything.
           if (!whole) hide(0u);
@@ -419,17 +421,22 @@ packed_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
           }
           mx = largest();
           const float size = fmaxf(mx, -fminf(min3(m4[0], m4[1], m4[2]), m4[3]));
-          if (!__any_sync(0xffffffffu, live && !(size * cap_x <= 1.f))) {
-            const uint64_t x2 = pack_f2(cap_x, cap_x), out2 = pack_f2(p.scale_log2, p.scale_log2);
+          const uint64_t x2 = pack_f2(cap_x, cap_x), out2 = pack_f2(p.scale_log2, p.scale_log2);
+          auto polynomial = [&](auto terms) {
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
               for (int c = 0; c < 32; c += 2) {
                 float a, b;
-                unpack_f2(soft_cap_small(pack_f2(__uint_as_float(sr[h][c]), __uint_as_float(sr[h][c + 1])), x2, out2), a, b);
+                unpack_f2(soft_cap_small<terms()>(pack_f2(__uint_as_float(sr[h][c]), __uint_as_float(sr[h][c + 1])), x2, out2), a, b);
                 sr[h][c] = __float_as_uint(a);
                 sr[h][c + 1] = __float_as_uint(b);
               }
+          };
+          if (!__any_sync(0xffffffffu, live && !(size * cap_x <= 0.25f))) {
+            polynomial(std::integral_constant<int, 3>{});
+          } else if (!__any_sync(0xffffffffu, live && !(size * cap_x <= 1.f))) {
+            polynomial(std::integral_constant<int, 7>{});
           } else {
 #pragma unroll
             for (int h = 0; h < 2; ++h)
@@ -632,8 +639,9 @@ packed_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
 template <typename T, int D, int MODE, int ROWS, bool CAP>
 static int launch_packed_x(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const PackedParams& p,
                            unsigned grid, cudaStream_t stream) {
-  return launch_in_clusters("packed_attention", packed_attention_kernel<T, D, MODE, ROWS, CAP>, dim3(grid * p.cluster), pa::THREADS,
-                            pa::Layout<D, ROWS>::SMEM_BYTES, p.cluster, false, stream, tq, tk, tv, p);
+  return launch_in_clusters<packed_attention_kernel<T, D, MODE, ROWS, CAP>>("packed_attention", dim3(grid * p.cluster), pa::THREADS,
+                                                                            pa::Layout<D, ROWS>::SMEM_BYTES, p.cluster, false,
+                                                                            stream, tq, tk, tv, p);
 }
 template <typename T, int D, int MODE>
 static int launch_packed_x(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const PackedParams& p,

@@ -42,34 +42,48 @@ def _dense(t):
     return t if t.stride(-1) == 1 or t.size(-1) == 1 else t.contiguous()
 
 
-def _check_output(out, x):
+def _output(out, x):
+    if out is None:
+        return torch.empty_like(x, memory_format=torch.contiguous_format)
     assert out.shape == x.shape and out.dtype is x.dtype and (out.stride(-1) == 1 or out.size(-1) == 1), \
         "q_embed / k_embed must have their input's shape and dtype, the last dimension contiguous"
+    return out
+
+
+def _rotated(q, k, positions, inv_freq, axes, inverse, q_out=None, k_out=None):
+    q, k = _dense(q), _dense(k)
+    q_out, k_out = _output(q_out, q), _output(k_out, k)
+    _launch(q, k, q_out, k_out, positions, inv_freq, axes, inverse)
+    return q_out, k_out
 
 
 class _MultiAxisRotary(torch.autograd.Function):
-    """The gradient of a rotation is the rotation back, so the backward pass is this function with the other sign (and
-    can be differentiated again)."""
+    """The gradient of a rotation is the rotation back, so the backward pass is the same launch with the other sign (and, where
+    it is to be differentiated again, this function)."""
 
     @staticmethod
     def forward(ctx, q, k, positions, inv_freq, axes, inverse):
         ctx.save_for_backward(positions, inv_freq)
         ctx.axes, ctx.inverse = axes, inverse
         ctx.set_materialize_grads(False)
-        q_out, k_out = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k))
-        _launch(_dense(q), _dense(k), q_out, k_out, positions, inv_freq, axes, inverse)
-        return q_out, k_out
+        return _rotated(q, k, positions, inv_freq, axes, inverse)
 
     @staticmethod
     def backward(ctx, grad_q, grad_k):
+        # an output that nothing was made of has no gradient, an input may want none: their heads are left out of the launch
+        if not ctx.needs_input_grad[0]:
+            grad_q = None
+        if not ctx.needs_input_grad[1]:
+            grad_k = None
         if grad_q is None and grad_k is None:
             return (None,) * 6
         positions, inv_freq = ctx.saved_tensors
-        # an output that nothing was made of has no gradient: its heads are left out of the launch
-        some = grad_k if grad_q is None else grad_q
-        none = some.new_empty((some.size(0), 0, some.size(2)))
-        dq, dk = _MultiAxisRotary.apply(none if grad_q is None else grad_q, none if grad_k is None else grad_k,
-                                        positions, inv_freq, ctx.axes, not ctx.inverse)
+        if grad_q is None or grad_k is None:
+            some = grad_k if grad_q is None else grad_q
+            none = some.new_empty((some.size(0), 0, some.size(2)))
+        rotate = _MultiAxisRotary.apply if torch.is_grad_enabled() else _rotated
+        dq, dk = rotate(none if grad_q is None else grad_q, none if grad_k is None else grad_k, positions, inv_freq,
+                        ctx.axes, not ctx.inverse)
         return None if grad_q is None else dq, None if grad_k is None else dk, None, None, None, None
 
 
@@ -110,14 +124,4 @@ def apply_multi_axis_rotary(
     if (q.requires_grad or k.requires_grad) and torch.is_grad_enabled():
         assert q_embed is None and k_embed is None, "outputs cannot be given where a gradient is wanted"
         return _MultiAxisRotary.apply(q, k, positions, inv_freq, axes, False)
-    q, k = _dense(q), _dense(k)
-    if q_embed is None:
-        q_embed = torch.empty_like(q, memory_format=torch.contiguous_format)
-    else:
-        _check_output(q_embed, q)
-    if k_embed is None:
-        k_embed = torch.empty_like(k, memory_format=torch.contiguous_format)
-    else:
-        _check_output(k_embed, k)
-    _launch(q, k, q_embed, k_embed, positions, inv_freq, axes, False)
-    return q_embed, k_embed
+    return _rotated(q, k, positions, inv_freq, axes, False, q_embed, k_embed)
