@@ -12,22 +12,24 @@ from torch import Tensor
 from .. import _lib
 from .sink_attention import check_paged, is64, rows_of_table
 
-# CTAs that run at a time, by the size of their clusters: a cluster stays inside a GPC, so that larger ones leave slots empty
-_SLOTS = {1: 296, 2: 296, 4: 280, 8: 256}
-
-
 @lru_cache(maxsize=256)
-def _pick_prefix_split(tiles: int, blocks: int):
-    """(tokens per split, CTAs per split) for `tiles` (row tile, kv head) pairs and `blocks` blocks of 64 keys.  In microseconds a
-    CTA takes about 0.7 for a block and 4 for the rest, a partial result 0.02 per pair (128 rows written and read again)
-    and 0.3 for its place in the join; the CTAs of a cluster join theirs among themselves in 1.  The shortest sum is taken."""
+def _pick_prefix_split(tiles: int, groups: int, hkv: int, blocks: int):
+    """(tokens per split, CTAs per split) for `tiles` (row tile, kv head) pairs of `groups` prefixes of up to `blocks` blocks of
+    64 keys, by the shortest sum, in microseconds: a block takes a CTA 1.0, beside another on its SM 1.1, or what memory needs
+    for it (32 KiB at 5.8 TB/s); a partial result 0.02 a pair (written and read again) and 0.3 for its place in the
+    join, joining a cluster 1.5; and past 224 CTAs (200 in clusters of four) no SM has room for the launch that follows, which otherwise goes through
+    the sequences' own tokens meanwhile: 10.  (8 pairs, 1876 blocks, with 128 / 192 / 224 / 288 / 384 CTAs: 129 / 113 / 114 /
+    136 / 124; 16 pairs, 512 blocks: 106 / 87 / 90 / 115 / 100.)  Clusters of two where prefixes differ in length, which splits
+    share out more evenly."""
+    memory = groups * hkv * blocks * 32768 / 5.8e6
     best, pick = None, (blocks, 1)
-    for cluster in (1, 2, 4, 8):
+    for cluster in (1, 2, 4) if groups == 1 else (1, 2):
         for splits in range(1, min(blocks, 64) + 1):
             per = -(-blocks // splits)
             splits = -(-blocks // per)
-            mine = -(-per // cluster)
-            cost = -(-tiles * splits * cluster // _SLOTS[cluster]) * (mine * 0.7 + 4 + (cluster > 1)) + splits * (0.02 * tiles + 0.3)
+            ctas = tiles * splits * cluster
+            work = -(-per // cluster) * -(-ctas // 280) * (1.0 if ctas <= 148 else 1.1)
+            cost = max(work, memory) + 1.5 * (cluster > 1) + splits * (0.02 * tiles + 0.3) + 10 * (ctas > (224 if cluster < 4 else 200))
             if best is None or cost < best:
                 best, pick = cost, (per, cluster)
     return pick[0] * 64, pick[1]
@@ -73,9 +75,9 @@ def shared_prefix_attention_fwd(
     wide = (is64(prefix_offsets, "prefix_offsets"), is64(prefix_seqlens, "prefix_seqlens"), is64(group_start, "group_start"),
             is64(block_offsets, "block_offsets"), is64(kv_seqlens, "kv_seqlens"))
     most = prefix_pages * page
-    heads = hq // hkv
-    tokens = (64 if -(-batch // groups) * heads <= 64 else 128) // heads              # to a row tile
-    chunk, cluster = _pick_prefix_split((batch // tokens + min(groups, batch)) * hkv, -(-most // 64))
+    heads, members = hq // hkv, -(-batch // groups)
+    tokens = (64 if members * heads <= 64 else 128) // heads                # to a row tile, as the launch has it
+    chunk, cluster = _pick_prefix_split(min(groups, batch) * -(-members // tokens) * hkv, groups, hkv, -(-most // 64))
     lib = _lib.load()
     with _lib.on_device(dev):
         floats = lib.dlb_shared_prefix_workspace_floats(batch, hq, max(dk, dv), -(-most // chunk))

@@ -152,10 +152,11 @@ def test_prefix_split_rule():
     """Chunks are whole blocks and no longer than the table; few rows are split over the SMs, many are not."""
     from dlcompiler_b200.kernels.shared_prefix_attention import _pick_prefix_split
 
-    for tiles in (1, 8, 64, 72, 296, 5000):
-        for blocks in (1, 2, 16, 63, 512, 1876, 30000):
-            chunk, cluster = _pick_prefix_split(tiles, blocks)
-            assert chunk % 64 == 0 and 64 <= chunk <= blocks * 64 and cluster in (1, 2, 4, 8)
-    assert _pick_prefix_split(5000, 512) == (512 * 64, 1)
-    chunk, cluster = _pick_prefix_split(8, 1876)
-    assert 8 * cluster * -(-1876 * 64 // chunk) > 148
+    for tiles in (0, 1, 8, 64, 72, 296, 5000):
+        for groups in (1, 3, 100):
+            for blocks in (1, 2, 16, 63, 512, 1876, 30000):
+                chunk, cluster = _pick_prefix_split(tiles, groups, 8, blocks)
+                assert chunk % 64 == 0 and 64 <= chunk <= blocks * 64 and cluster in (1, 2, 4)
+    assert _pick_prefix_split(5000, 1, 8, 512) == (512 * 64, 1)
+    chunk, cluster = _pick_prefix_split(8, 1, 8, 1876)
+    assert 148 < 8 * cluster * -(-1876 * 64 // chunk) <= 224
