@@ -77,30 +77,39 @@ struct PackedParams {
   PrefixPartials prefix;          // PREFIX
 };
 
-// Row tile x of the launch -> sequence (or group) and tile inside it, its rows and keys; false if there is none.  The tiles
-// that exist are numbered through, sequence by sequence, 32 sequences at a time over the lanes of a warp (every warp does it
-// for itself), so that a batch of any lengths needs no more CTAs than it has tiles.
+// First row, number of rows and number of keys of sequence (or group) b; rows outside q are nobody's.
 template <int MODE>
+__device__ __forceinline__ void packed_rows(const PackedParams& p, int b, int& start, int& n, int& kv_len) {
+  if (MODE == pa::PREFIX) {
+    group_rows(p.prefix, p.tokens, b, start, n);
+    kv_len = load_index(p.prefix.lens, b, p.prefix.lens_is_int64);
+  } else {
+    start = load_index(p.q_start, b, p.start_is_int64);
+    n = load_index(p.q_lens, b, p.qlens_is_int64);
+    kv_len = load_index(p.kv_lens, b, p.lens_is_int64);
+    n = (start < 0 || start >= p.tokens) ? 0 : (int)min((int64_t)max(n, 0), p.tokens - start);
+  }
+}
+
+// Row tile x of the launch -> sequence (or group) and tile inside it, its rows and keys; false if there is none.  The tiles
+// that exist are numbered through, sequence by sequence, so that a batch of any lengths needs no more CTAs than it has tiles.
+// Every warp counts for itself: a lane has EACH sequences, one where 32 lanes are enough for the batch (its sizes are then at
+// hand when it is found), else four, so that few loads wait for one another.
+template <int MODE, int EACH>
 __device__ __forceinline__ bool packed_tile(const PackedParams& p, int x, int& seq, int& tile, int& start, int& n, int& kv_len) {
   const int lane = threadIdx.x & 31;
   int before = 0;
-  for (int b0 = 0; b0 < p.batch; b0 += 32) {
-    const int b = b0 + lane;
-    int st = 0, rows = 0, keys = 0;
-    if (b < p.batch) {
-      if (MODE == pa::PREFIX) {
-        group_rows(p.prefix, p.tokens, b, st, rows);
-        keys = load_index(p.prefix.lens, b, p.prefix.lens_is_int64);
-      } else {
-        // rows outside q are nobody's
-        st = load_index(p.q_start, b, p.start_is_int64);
-        rows = load_index(p.q_lens, b, p.qlens_is_int64);
-        keys = load_index(p.kv_lens, b, p.lens_is_int64);
-        rows = (st < 0 || st >= p.tokens) ? 0 : (int)min((int64_t)max(rows, 0), p.tokens - st);
-      }
+  for (int b0 = 0; b0 < p.batch; b0 += 32 * EACH) {
+    int mine[EACH], all = 0, st = 0, rows = 0, keys = 0;
+#pragma unroll
+    for (int u = 0; u < EACH; ++u) {
+      const int b = b0 + lane * EACH + u;
+      rows = 0;
+      if (b < p.batch) packed_rows<MODE>(p, b, st, rows, keys);
+      mine[u] = (rows + p.tile_tokens - 1) / p.tile_tokens;
+      all += mine[u];
     }
-    const int mine = (rows + p.tile_tokens - 1) / p.tile_tokens;
-    int upto = mine;
+    int upto = all;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int v = __shfl_up_sync(0xffffffffu, upto, o);
@@ -109,12 +118,25 @@ __device__ __forceinline__ bool packed_tile(const PackedParams& p, int x, int& s
     const uint32_t past = __ballot_sync(0xffffffffu, before + upto > x);
     if (past != 0) {
       const int src = __ffs(past) - 1;
-      seq = b0 + src;
-      const int of_seq = __shfl_sync(0xffffffffu, mine, src);
-      tile = of_seq - 1 - (x - (before + __shfl_sync(0xffffffffu, upto, src) - of_seq));   // the late, long ones first
-      start = __shfl_sync(0xffffffffu, st, src);
-      n = __shfl_sync(0xffffffffu, rows, src);
-      kv_len = __shfl_sync(0xffffffffu, keys, src);
+      int at = before + __shfl_sync(0xffffffffu, upto - all, src), of_seq = 0;     // tiles in front of the lane's first sequence
+      seq = b0 + src * EACH - 1;
+#pragma unroll
+      for (int u = 0; u < EACH; ++u) {
+        const int m = __shfl_sync(0xffffffffu, mine[u], src);
+        if (at + of_seq <= x) {
+          at += of_seq;
+          of_seq = m;
+          ++seq;
+        }
+      }
+      tile = of_seq - 1 - (x - at);                       // the late, long ones first
+      if (EACH == 1) {
+        start = __shfl_sync(0xffffffffu, st, src);
+        n = __shfl_sync(0xffffffffu, rows, src);
+        kv_len = __shfl_sync(0xffffffffu, keys, src);
+      } else {
+        packed_rows<MODE>(p, seq, start, n, kv_len);
+      }
       return true;
     }
     before += __shfl_sync(0xffffffffu, upto, 31);
@@ -147,7 +169,8 @@ packed_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
   }
   if (MODE == PREFIX) let_next_start();
   int seq, tile, start, n, kv_len;
-  if (!packed_tile<MODE>(p, x, seq, tile, start, n, kv_len)) return;
+  if (!(p.batch <= 32 ? packed_tile<MODE, 1>(p, x, seq, tile, start, n, kv_len) : packed_tile<MODE, 4>(p, x, seq, tile, start, n, kv_len)))
+    return;
   const int q0 = tile * p.tile_tokens;
   const int tile_rows = min(p.tile_tokens, n - q0) * p.group;        // rows of this tile that exist
   const int hist = kv_len - (MODE == PREFILL ? load_index(p.q_lens, seq, p.qlens_is_int64) : 0);
@@ -676,7 +699,7 @@ static int check_attention(const char* what, int64_t batch, int64_t tokens, int6
   DLB_CHECK_ARG(batch >= 0 && tokens >= 0 && hq >= 1 && hkv >= 1 && hq % hkv == 0, DLB_ERR_BAD_ARG, "%s: bad sizes", what);
   DLB_CHECK_ARG(hq / hkv <= pa::BM, DLB_ERR_UNSUPPORTED, "%s: %lld q-heads to a kv head (at most %d)", what,
                 (long long)(hq / hkv), pa::BM);
-  DLB_CHECK_ARG(page_size >= 16 && page_size <= 65536 && (page_size & (page_size - 1)) == 0, DLB_ERR_UNSUPPORTED,
+  DLB_CHECK_ARG(page_size >= 16 && page_size <= (1 << 30) && (page_size & (page_size - 1)) == 0, DLB_ERR_UNSUPPORTED,
                 "%s: page size %lld must be a power of two from 16 on", what, (long long)page_size);
   DLB_CHECK_ARG(num_pages >= 1 && max_pages >= 1, DLB_ERR_BAD_ARG, "%s: empty cache or table", what);
   DLB_CHECK_ARG(num_pages < (1LL << 31) && max_pages * page_size < (1LL << 31) && tokens * hq < (1LL << 31) &&
@@ -818,7 +841,7 @@ extern "C" int dlb_shared_prefix_attention(
   int rc = check_attention("shared_prefix_attention", batch, batch, hq, hkv, head_dim, head_dim_v, page_size, num_pages,
                            max_pages < prefix_max_pages ? max_pages : prefix_max_pages, sm_scale, dtype, width);
   if (rc != DLB_OK) return rc;
-  DLB_CHECK_ARG(groups >= 1 && groups <= batch + 65535 && prefix_max_pages * page_size < (1LL << 31) &&
+  DLB_CHECK_ARG(groups >= 1 && groups <= 65535 && prefix_max_pages * page_size < (1LL << 31) &&
                     max_pages * page_size < (1LL << 31),
                 DLB_ERR_TOO_LARGE, "shared_prefix_attention: number of groups or length of a table out of range");
   DLB_CHECK_ARG(chunk >= 64 && chunk % 64 == 0 && chunk < (1LL << 31), DLB_ERR_BAD_ARG,

@@ -35,6 +35,11 @@ def _pick_prefix_split(tiles: int, groups: int, hkv: int, blocks: int):
     return pick[0] * 64, pick[1]
 
 
+@lru_cache(maxsize=256)
+def _workspace_floats(*sizes):
+    return _lib.load().dlb_shared_prefix_workspace_floats(*sizes)
+
+
 def shared_prefix_attention_fwd(
     q: Tensor,
     k: Tensor,
@@ -80,8 +85,7 @@ def shared_prefix_attention_fwd(
     chunk, cluster = _pick_prefix_split(min(groups, batch) * -(-members // tokens) * hkv, groups, hkv, -(-most // 64))
     lib = _lib.load()
     with _lib.on_device(dev):
-        floats = lib.dlb_shared_prefix_workspace_floats(batch, hq, max(dk, dv), -(-most // chunk))
-        partial = torch.empty(floats, dtype=torch.float32, device=dev)
+        partial = torch.empty(_workspace_floats(batch, hq, max(dk, dv), -(-most // chunk)), dtype=torch.float32, device=dev)
         rc = lib.dlb_shared_prefix_attention(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), prefix_offsets.data_ptr(),
             prefix_seqlens.data_ptr(), group_start.data_ptr(), block_offsets.data_ptr(), kv_seqlens.data_ptr(),

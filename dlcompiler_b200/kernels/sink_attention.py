@@ -46,7 +46,7 @@ def check_paged(q: Tensor, k: Tensor, v: Tensor, o: Tensor):
     (q_st, q_sh, q_last), (o_st, o_sh, o_last) = q.stride(), o.stride()
     (*k_strides, k_last), (*v_strides, v_last) = k.stride(), v.stride()
     assert k_last == 1 and v_last == 1 and o_last == 1, "the last dimension must be contiguous"
-    if q_last != 1 or q_st % 8 or q_sh % 8 or q.data_ptr() % 16:
+    if q_last != 1 or q_st % 8 or q_sh % 8 or not (q_st and q_sh) or q.data_ptr() % 16:
         q = q.clone(memory_format=torch.contiguous_format)
         q_st, q_sh = hq * dk, dk
     return q, (tokens, hq, hkv, dk, dv, page, pages), (q_st, q_sh, o_st, o_sh, *k_strides, *v_strides)
@@ -97,7 +97,7 @@ def sink_attention_fwd(
         rc = lib.dlb_sink_attention(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), block_offsets.data_ptr(), q_start_loc.data_ptr(),
             q_seqlens.data_ptr(), kv_seqlens.data_ptr(), batch, tokens, int(max_seqlen), hq, hkv, dk, dv, page, pages,
-            columns, *strides, bt_stride, *wide, int(window_size), int(num_sinks), dk ** -0.5 if sm_scale is None else sm_scale,
+            columns, *strides, bt_stride, *wide, min(int(window_size), 2**31), min(int(num_sinks), 2**31), dk ** -0.5 if sm_scale is None else sm_scale,
             logit_softcapping or -1.0, _lib.dtype_code(q), _lib.status_word(dev).data_ptr(), _lib.stream_ptr(dev))
     _lib.check(rc, "sink_attention_fwd")
     return o

@@ -73,6 +73,7 @@ CASES = [  # members, prefix, own, page, hq, hkv, d, dv, dtype, cap
     ([70], [2500], [i % 7 for i in range(70)], 32, 8, 8, 128, 64, BF, 30.0),
     ([1, 1, 1], [0, 0, 63], [0, 70, 0], 128, 40, 1, 40, 128, BF, 0.0),
     ([4] * 40, [50 + 3 * i for i in range(40)], [1 + i % 50 for i in range(160)], 16, 4, 2, 64, 64, BF, 0.0),
+    ([i % 3 for i in range(150)], [20 + i for i in range(150)], [1 + i % 20 for i in range(150)], 16, 4, 2, 64, 64, BF, 0.0),
     ([3, 2], [300, 200], [900, 5, 2000, 64, 63], 256, 128, 1, 72, 72, FP, 10.0),
     ([2], [40000], [3, 700], 64, 32, 8, 128, 128, BF, 0.0),
     ([150], [700], [5] * 150, 64, 16, 16, 64, 64, FP, 0.0),

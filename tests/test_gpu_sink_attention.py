@@ -119,6 +119,7 @@ SEVERAL = [  # new, past, window, sinks, page, hq, hkv, d, dv, dtype, cap
     ([31], [900], 300, 1, 256, 128, 1, 64, 128, FP, 0.0),
     ([40], [90], 17, 3, 16, 100, 1, 40, 48, BF, 15.0),
     ([7] * 40, [13 * i for i in range(40)], 100, 5, 16, 4, 2, 64, 64, BF, 0.0),
+    ([(5 * i) % 4 for i in range(301)], [7 * i % 90 for i in range(301)], 40, 5, 16, 4, 2, 64, 64, BF, 0.0),
     ([1500], [0], 700, 4, 64, 8, 2, 128, 128, BF, 0.0),
     ([5, 2, 9], [5000, 700, 0], 4095, 4, 16, 28, 4, 128, 128, FP, 0.0),
     ([3], [2500], 1023, 70, 64, 4, 4, 64, 64, BF, 20.0),
