@@ -1,0 +1,136 @@
+"""GPU: the serving operators together, as a server calls them: rotary positions of several axes for q and k, the keys and
+values into the paged cache, attention over it, with a window and sinks or behind a shared prefix."""
+import pytest
+import torch
+
+from dlcompiler_b200 import (apply_multi_axis_rotary, check_device_status, fill_kv_cache, paged_attention_fwd,
+                             shared_prefix_attention_fwd, sink_attention_fwd)
+from tests.paged_reference import attend, close, rows_of
+
+pytestmark = pytest.mark.gpu
+HQ, HKV, D, PAGE, SECTIONS = 8, 2, 64, 16, [8, 12, 12]
+
+
+def _ints(x, dev):
+    return torch.tensor(x, dtype=torch.int32, device=dev)
+
+
+class Server:
+    def __init__(self, dev, batch, pages, columns, dtype, seed):
+        self.dev, self.g = dev, torch.Generator().manual_seed(seed)
+        self.k, self.v = (torch.full((pages, PAGE, HKV, D), float("nan"), dtype=dtype, device=dev) for _ in range(2))
+        self.free = torch.randperm(pages, generator=self.g).tolist()
+        self.table = torch.full((batch, columns), -1, dtype=torch.int32, device=dev)
+        self.inv = (10000.0 ** (-torch.arange(D // 2, dtype=torch.float64) / (D // 2))).float().to(dev)
+        self.dtype = dtype
+
+    def need(self, table, row, tokens):
+        for c in range(-(-tokens // PAGE)):
+            if int(table[row, c]) < 0:
+                table[row, c] = self.free.pop()
+
+    def project(self, tokens):
+        qkv = torch.randn(tokens, (HQ + 2 * HKV) * D, generator=self.g).to(self.dtype).to(self.dev)
+        return [t.view(tokens, -1, D) for t in qkv.split([HQ * D, HKV * D, HKV * D], 1)]
+
+    def rotated(self, q, k, positions):
+        return apply_multi_axis_rotary(q, k, positions.to(self.dev), self.inv, SECTIONS)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_prompts_with_images_then_tokens_behind_a_window(cuda_device, dtype):
+    """Prompts (a grid of patches between text), drafted tokens and single ones; pages behind the window are given back and
+    their entries go stale, so that other sequences' tokens land there."""
+    window, sinks, lens = 40, 5, [70, 33, 1]
+    s = Server(cuda_device, 3, 24, 12, dtype, 1)
+    grid = torch.cartesian_prod(torch.arange(2), torch.arange(4), torch.arange(3)).t()
+    done = [0, 0, 0]
+    keys, values = [[], [], []], [[], [], []]
+    for step, new in enumerate([lens, [4, 2, 3]] + [[1, 1, 1]] * 6):
+        total = sum(new)
+        q, k, v = s.project(total)
+        pos = []
+        for b, n in enumerate(new):
+            p = (done[b] + torch.arange(n)).repeat(3, 1)
+            if step == 0 and n > 40:
+                p[:, 5:29] = 5 + grid
+            pos.append(p)
+            done[b] += n
+            s.need(s.table, b, done[b])
+        q, k = s.rotated(q, k, torch.cat(pos, 1))
+        start = _ints([0, new[0], new[0] + new[1]], s.dev)
+        args = (start, _ints(new, s.dev), _ints(done, s.dev), max(new))
+        fill_kv_cache(k, v, s.k, s.v, *args, s.table)
+        o = torch.empty_like(q)
+        sink_attention_fwd(q, s.k, s.v, o, s.table, *args, window, sinks)
+        at = 0
+        for b, n in enumerate(new):
+            keys[b].append(k[at:at + n])
+            values[b].append(v[at:at + n])
+            kk, vv = torch.cat(keys[b]), torch.cat(values[b])
+            row, key = torch.arange(done[b] - n, done[b], device=s.dev)[:, None], torch.arange(done[b], device=s.dev)
+            seen = (key <= row) & ((key >= row - window) | (key < sinks))
+            ref, bound = attend(q[at:at + n], kk, vv, seen, D ** -0.5, 0.0, dtype)
+            close(o[at:at + n], ref, bound, f"step {step}, sequence {b}")
+            at += n
+            # what no later token sees is given back
+            for c in range(-(-sinks // PAGE), (done[b] - window) // PAGE):
+                if int(s.table[b, c]) >= 0:
+                    s.free.append(int(s.table[b, c]))
+                    s.table[b, c] = -1
+    check_device_status()
+
+
+def test_answers_behind_one_prompt_in_a_graph(cuda_device):
+    """The prompt once, then a step of all answers captured into a graph and replayed: each like paged_attention_fwd over the
+    whole context, whose pages the prompt fills."""
+    dtype, prompt, batch, steps = torch.bfloat16, 96, 5, 20
+    s = Server(cuda_device, batch, 40, 3, dtype, 2)
+    prefix = torch.full((1, prompt // PAGE), -1, dtype=torch.int32, device=s.dev)
+    s.need(prefix, 0, prompt)
+    for b in range(batch):
+        s.need(s.table, b, steps + 1)
+    q, k, v = s.project(prompt)
+    q, k = s.rotated(q, k, torch.arange(prompt).repeat(3, 1))
+    fill_kv_cache(k, v, s.k, s.v, _ints([0], s.dev), _ints([prompt], s.dev), _ints([prompt], s.dev), prompt, prefix)
+    qkv = torch.zeros(batch, (HQ + 2 * HKV) * D, dtype=dtype, device=s.dev)
+    q, k, v = (t.view(batch, -1, D) for t in qkv.split([HQ * D, HKV * D, HKV * D], 1))
+    pos = torch.full((3, batch), prompt, dtype=torch.int64, device=s.dev)
+    own, one, start = _ints([1] * batch, s.dev), _ints([1] * batch, s.dev), _ints(list(range(batch)), s.dev)
+    plen, groups = _ints([prompt], s.dev), _ints([0, batch], s.dev)
+    o = torch.empty(batch, HQ, D, dtype=dtype, device=s.dev)
+
+    def step():
+        qr, kr = apply_multi_axis_rotary(q, k, pos, s.inv, SECTIONS)
+        fill_kv_cache(kr, v, s.k, s.v, start, one, own, 1, s.table)
+        shared_prefix_attention_fwd(qr, s.k, s.v, o, prefix, plen, groups, s.table, own)
+        return qr
+
+    s.k.nan_to_num_(0.0), s.v.nan_to_num_(0.0)
+    step()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        qr = step()
+    whole = torch.cat([prefix.expand(batch, -1), s.table], 1).contiguous()
+    other = torch.empty_like(o)
+    for t in range(steps):
+        qkv.copy_(torch.randn(qkv.shape, generator=s.g).to(dtype))
+        own.fill_(t + 1)
+        pos.fill_(prompt + t)
+        graph.replay()
+        got = o.clone()
+        assert torch.equal(got, shared_prefix_attention_fwd(qr, s.k, s.v, torch.empty_like(o), prefix, plen, groups, s.table, own))
+        paged_attention_fwd(qr, s.k, s.v, other, whole, start, one, own + prompt, 1)
+        kk, vv = s.k.view(-1, HKV, D), s.v.view(-1, HKV, D)
+        for b in range(batch):
+            rows = rows_of(whole[b], prompt + t + 1, PAGE)
+            seen = torch.ones(1, rows.numel(), dtype=torch.bool, device=s.dev)
+            ref, bound = attend(qr[b:b + 1], kk[rows], vv[rows], seen, D ** -0.5, 0.0, dtype)
+            close(got[b:b + 1], ref, bound, f"step {t}, sequence {b}")
+            close(other[b:b + 1], ref, bound, f"whole context, step {t}, sequence {b}")
+    check_device_status()
