@@ -79,19 +79,30 @@ __device__ __forceinline__ float soft_cap(float s, float in, float out) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + fast_exp2(s * in)));
   return fmaf(-2.f * out, r, out);
 }
-// The same for |x| <= 1 (TERMS = 7) or 1/4 (3) without the special-function unit: tanh(x) = x P(x^2), P interpolated at the
-// Chebyshev nodes of [0, 1] or [0, 1/16], off by 1.2e-7 (2^-23) with 32-bit coefficients.  Two scores at a time:
-// `x` = sm_scale / cap, `out` = sm_scale log2(e).
-template <int TERMS> __device__ __forceinline__ uint64_t soft_cap_small(uint64_t s, uint64_t x, uint64_t out) {
-  constexpr float P7[7] = {0.99999995f, -0.33332828f, 0.13325076f, -0.05345165f, 0.02027971f, -0.00619432f, 0.00103803f};
-  constexpr float P3[3] = {0.99999958f, -0.33321896f, 0.12841433f};
+// The same without the special-function unit: tanh(x) = x P(x^2), P interpolated at the Chebyshev nodes, off by 1.2e-7 (2^-23)
+// with 32-bit coefficients, for |x| <= 1 (7 terms) or 1/4 (3).  Two scores at a time; x = sm_scale / cap goes into the
+// argument of the long form and, once for a row, into the coefficients of the short one.
+__device__ __forceinline__ uint64_t soft_cap_below(uint64_t s, uint64_t x, uint64_t out) {     // out = sm_scale log2(e)
+  constexpr float P[7] = {0.99999995f, -0.33332828f, 0.13325076f, -0.05345165f, 0.02027971f, -0.00619432f, 0.00103803f};
   const uint64_t u1 = mul_f2(s, x), u = mul_f2(u1, u1);
-  auto term = [](int i) { return TERMS == 7 ? pack_f2(P7[i], P7[i]) : pack_f2(P3[i % 3], P3[i % 3]); };
-  uint64_t p = term(TERMS - 1);
+  uint64_t p = pack_f2(P[6], P[6]);
 #pragma unroll
-  for (int i = TERMS - 2; i >= 0; --i) p = fma_f2(p, u, term(i));
+  for (int i = 5; i >= 0; --i) p = fma_f2(p, u, pack_f2(P[i], P[i]));
   return mul_f2(mul_f2(s, out), p);
 }
+struct SoftCapShort {
+  uint64_t c0, c1, c2;
+  __device__ __forceinline__ SoftCapShort(float x, float out) {
+    const float a = 0.99999958f * out, b = -0.33321896f * out * (x * x), c = 0.12841433f * out * (x * x) * (x * x);
+    c0 = pack_f2(a, a);
+    c1 = pack_f2(b, b);
+    c2 = pack_f2(c, c);
+  }
+  __device__ __forceinline__ uint64_t operator()(uint64_t s) const {
+    const uint64_t u = mul_f2(s, s);
+    return mul_f2(s, fma_f2(fma_f2(c2, u, c1), u, c0));
+  }
+};
 
 __device__ __forceinline__ void cluster_barrier() {
   asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");

@@ -23,8 +23,6 @@
 // that hold no key which the tile sees.
 #include <math_constants.h>
 
-#include <type_traits>
-
 #include "cluster_decode.cuh"
 
 namespace dlb {
@@ -444,22 +442,22 @@ packed_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
           }
           mx = largest();
           const float size = fmaxf(mx, -fminf(min3(m4[0], m4[1], m4[2]), m4[3]));
-          const uint64_t x2 = pack_f2(cap_x, cap_x), out2 = pack_f2(p.scale_log2, p.scale_log2);
-          auto polynomial = [&](auto terms) {
+          auto each_pair = [&](auto&& f) {
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
               for (int c = 0; c < 32; c += 2) {
                 float a, b;
-                unpack_f2(soft_cap_small<terms()>(pack_f2(__uint_as_float(sr[h][c]), __uint_as_float(sr[h][c + 1])), x2, out2), a, b);
+                unpack_f2(f(pack_f2(__uint_as_float(sr[h][c]), __uint_as_float(sr[h][c + 1]))), a, b);
                 sr[h][c] = __float_as_uint(a);
                 sr[h][c + 1] = __float_as_uint(b);
               }
           };
-          if (!__any_sync(0xffffffffu, live && !(size * cap_x <= 0.25f))) {
-            polynomial(std::integral_constant<int, 3>{});
+          if (cap_x <= 1e8f && !__any_sync(0xffffffffu, live && !(size * cap_x <= 0.25f))) {     // x^4 is a number
+            each_pair(SoftCapShort(cap_x, p.scale_log2));
           } else if (!__any_sync(0xffffffffu, live && !(size * cap_x <= 1.f))) {
-            polynomial(std::integral_constant<int, 7>{});
+            const uint64_t x2 = pack_f2(cap_x, cap_x), out2 = pack_f2(p.scale_log2, p.scale_log2);
+            each_pair([&](uint64_t v) { return soft_cap_below(v, x2, out2); });
           } else {
 #pragma unroll
             for (int h = 0; h < 2; ++h)
