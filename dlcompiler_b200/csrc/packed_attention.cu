@@ -721,14 +721,17 @@ static int log2_of(int64_t v) {
   return s;
 }
 
-// CTAs to a (row tile, kv head).  In microseconds a CTA takes about 4 for everything but its blocks, 2 more for a join, and for
-// a block 0.6 alone on its SM and 0.9 beside another; the shortest sum over the waves is taken.
+// CTAs to a (row tile, kv head), for `pairs` of them with up to `blocks` blocks.  In microseconds a CTA takes about 4 for everything
+// but its blocks, 2 more for a join, and for a block 0.6 alone on its SM and 0.9 beside another.  Clusters only where all of
+// them run at once: behind a first wave each costs about 10 more.  Measured with 1 / 2 / 4 / 8 (us, 4 heads to a kv head, 128 columns):
+//    64 pairs of 65 blocks  58.3 / 40.1 / 30.8 / 44.5      128 pairs of 65 blocks  58.8 / 48.2 / 56.8 / 83.1
+//    64 pairs of  4 blocks  10.1 / 15.2 / 13.4 / 26.0      256 pairs of 65 blocks  71.0 / 71.7 / 89.7 / 140.7
+//   640 pairs of 17 blocks  76.7 / 120 / 168 / 323        1024 pairs of 1 to 64     132 / 202 / 286 / 499
 static int pick_packed_cluster(int64_t pairs, int64_t blocks) {
   int best = 1;
   int64_t best_cost = INT64_MAX;
-  for (int c = 1; c <= MAX_CLUSTER; c *= 2) {
-    const int64_t slots = cluster_slots(c), ctas = pairs * c;
-    const int64_t cost = (ctas + slots - 1) / slots * ((blocks + c - 1) / c * (2 * ctas <= slots ? 6 : 9) + 40 + (c > 1 ? 20 : 0));
+  for (int c = 1; c <= MAX_CLUSTER && (c == 1 || pairs * c <= cluster_slots(c)); c *= 2) {
+    const int64_t cost = (blocks + c - 1) / c * (2 * pairs * c <= cluster_slots(c) ? 6 : 9) + 40 + (c > 1 ? 20 : 0);
     if (cost < best_cost) {
       best = c;
       best_cost = cost;
@@ -805,7 +808,8 @@ extern "C" int dlb_sink_attention(const void* q, const void* k_cache, const void
   DLB_CHECK_ARG(tiles * hkv * MAX_CLUSTER < (1LL << 31), DLB_ERR_TOO_LARGE, "sink_attention: grid too large");
   p.tiles = (int)tiles;
   const int64_t seen = window + p.tile_tokens + sinks < max_pages * page_size ? window + p.tile_tokens + sinks : max_pages * page_size;
-  p.cluster = pick_packed_cluster(tiles * hkv, (seen + pa::BN - 1) / pa::BN);
+  const int64_t likely = batch * ((total_q_tokens / batch + p.tile_tokens - 1) / p.tile_tokens);      // with sequences of one length
+  p.cluster = pick_packed_cluster((likely < tiles ? likely : tiles) * hkv, (seen + pa::BN - 1) / pa::BN);
   CUtensorMap tq, tk, tv;
   rc = make_tmap_tokens(&tq, q, head_dim, hq, total_q_tokens, q_stride_h, q_stride_t, p.tile_tokens, p.group);
   if (rc != DLB_OK) return rc;

@@ -12,15 +12,17 @@ from torch import Tensor
 from .. import _lib
 from .sink_attention import check_paged, is64, rows_of_table
 
+
 @lru_cache(maxsize=256)
 def _pick_prefix_split(tiles: int, groups: int, hkv: int, blocks: int):
     """(tokens per split, CTAs per split) for `tiles` (row tile, kv head) pairs of `groups` prefixes of up to `blocks` blocks of
     64 keys, by the shortest sum, in microseconds: a block takes a CTA 1.0, beside another on its SM 1.1, or what memory needs
-    for it (32 KiB at 5.8 TB/s); a partial result 0.02 a pair (written and read again) and 0.3 for its place in the
-    join, joining a cluster 1.5; and past 224 CTAs (200 in clusters of four) no SM has room for the launch that follows, which otherwise goes through
-    the sequences' own tokens meanwhile: 10.  (8 pairs, 1876 blocks, with 128 / 192 / 224 / 288 / 384 CTAs: 129 / 113 / 114 /
-    136 / 124; 16 pairs, 512 blocks: 106 / 87 / 90 / 115 / 100.)  Clusters of two where prefixes differ in length, which splits
-    share out more evenly."""
+    for it (32 KiB at 5.8 TB/s); every wave of CTAs 4, in clusters 10 more behind the first one; a partial result 0.02 a pair
+    (written and read again) and 0.3 for its place in the join, joining a cluster 1.5; and past 224 CTAs (200 in clusters of
+    four) no SM has room for the launch that follows, which otherwise goes through the sequences' own tokens meanwhile: 10.
+    (8 pairs, 1876 blocks, with 128 / 192 / 224 / 288 / 384 CTAs: 129 / 113 / 114 / 136 / 124; 16 pairs, 512 blocks: 106 / 87 /
+    90 / 115 / 100.  256 pairs, 313 blocks, whole / in 4 splits / in 3 splits of clusters of four: 417 / 445 / 512.)  Clusters
+    of two where prefixes differ in length, which splits share out more evenly."""
     memory = groups * hkv * blocks * 32768 / 5.8e6
     best, pick = None, (blocks, 1)
     for cluster in (1, 2, 4) if groups == 1 else (1, 2):
@@ -28,8 +30,10 @@ def _pick_prefix_split(tiles: int, groups: int, hkv: int, blocks: int):
             per = -(-blocks // splits)
             splits = -(-blocks // per)
             ctas = tiles * splits * cluster
-            work = -(-per // cluster) * -(-ctas // 280) * (1.0 if ctas <= 148 else 1.1)
-            cost = max(work, memory) + 1.5 * (cluster > 1) + splits * (0.02 * tiles + 0.3) + 10 * (ctas > (224 if cluster < 4 else 200))
+            waves = -(-ctas // 280)
+            work = waves * (-(-per // cluster) * (1.0 if ctas <= 148 else 1.1) + 4) + 10 * (waves - 1) * (cluster > 1)
+            cost = max(work, memory + 4) + 1.5 * (cluster > 1) + splits * (0.02 * tiles + 0.3) \
+                + 10 * (ctas > (224 if cluster < 4 else 200))
             if best is None or cost < best:
                 best, pick = cost, (per, cluster)
     return pick[0] * 64, pick[1]
