@@ -235,7 +235,9 @@ cluster_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
       if (lane == 0) *ext_splits = n;
     }
     const float scale2 = p.sm_scale * 1.4426950408889634f;
-    const float cap_in = CAP ? 2.f * 1.4426950408889634f * p.sm_scale / p.softcap : 0.f, cap_out = p.softcap * 1.4426950408889634f;
+    const float cap_in = CAP ? 2.f * 1.4426950408889634f * p.sm_scale / p.softcap : 0.f, cap_out = p.softcap * 1.4426950408889634f,
+                cap_x = CAP ? p.sm_scale / p.softcap : 0.f;
+    const SoftCapShort cap_short(cap_x, scale2);
     const int mat = lane >> 3;      // ldmatrix: which 8x8 matrix this lane addresses
     const int mrow = lane & 7;
 
@@ -285,11 +287,13 @@ cluster_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
       bool grow = false;
 #pragma unroll
       for (int n = 0; n < NH; ++n) {
+        if (CAP) {
+          soft_cap_any(sacc[n][0], sacc[n][1], cap_short, cap_x, cap_in, cap_out);
+          soft_cap_any(sacc[n][2], sacc[n][3], cap_short, cap_x, cap_in, cap_out);
+        }
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-          float v = sacc[n][u];
-          if (CAP) v = soft_cap(v, cap_in, cap_out);
-          else v *= scale2;
+          float v = CAP ? sacc[n][u] : sacc[n][u] * scale2;
           if (partly) {
             const int key = key0 + (lane >> 2) + (u >> 1) * 8;
             v = (key >= from && key < to) ? v : -CUDART_INF_F;
@@ -328,8 +332,8 @@ cluster_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
         float e[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-          const float mref = m_run[n][u & 1];
-          e[u] = mref == -CUDART_INF_F ? 0.f : fast_exp2(sacc[n][u] - mref);
+          const float mref = m_run[n][u & 1];                  // -inf: no score so far but -inf, or one that is no number
+          e[u] = fast_exp2(mref == -CUDART_INF_F ? sacc[n][u] : sacc[n][u] - mref);
           l_run[n][u & 1] += e[u];
         }
         pf[n][0] = transpose_8x8(pack_pair<T>(e[0], e[1]));

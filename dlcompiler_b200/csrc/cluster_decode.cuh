@@ -73,15 +73,16 @@ __device__ __forceinline__ void group_rows(const PrefixPartials& p, int64_t toke
 }
 
 // cap * tanh(x) in the base-2 domain from one exponential and one reciprocal: tanh(x) = 1 - 2 / (1 + e^2x).  Off by 2^-22 of
-// the cap, like a score of that size; `in` = 2 log2(e) sm_scale / cap, `out` = cap log2(e).
+// the cap, so for scores that come near it; `in` = 2 log2(e) sm_scale / cap, `out` = cap log2(e).
 __device__ __forceinline__ float soft_cap(float s, float in, float out) {
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + fast_exp2(s * in)));
   return fmaf(-2.f * out, r, out);
 }
-// The same without the special-function unit: tanh(x) = x P(x^2), P interpolated at the Chebyshev nodes, off by 1.2e-7 (2^-23)
-// with 32-bit coefficients, for |x| <= 1 (7 terms) or 1/4 (3).  Two scores at a time; x = sm_scale / cap goes into the
-// argument of the long form and, once for a row, into the coefficients of the short one.
+// The same without the special-function unit: tanh(x) = x P(x^2), P interpolated at the Chebyshev nodes, off by 2^-21 of the
+// score with 32-bit coefficients (a score is a sum of up to 128 rounded products), for |x| <= 1 (7 terms) or 1/4 (3).  Two
+// scores at a time; x = sm_scale / cap goes into the argument of the long form and, once for a row, into the coefficients
+// of the short one.
 __device__ __forceinline__ uint64_t soft_cap_below(uint64_t s, uint64_t x, uint64_t out) {     // out = sm_scale log2(e)
   constexpr float P[7] = {0.99999995f, -0.33332828f, 0.13325076f, -0.05345165f, 0.02027971f, -0.00619432f, 0.00103803f};
   const uint64_t u1 = mul_f2(s, x), u = mul_f2(u1, u1);
@@ -103,6 +104,14 @@ struct SoftCapShort {
     return mul_f2(s, fma_f2(fma_f2(c2, u, c1), u, c0));
   }
 };
+
+// Two scores of any size: the small ones by the polynomial, since the other way is off by 2^-22 of the cap, however large that is.
+__device__ __forceinline__ void soft_cap_any(float& a, float& b, const SoftCapShort& low, float x, float in, float out) {
+  float la, lb;
+  unpack_f2(low(pack_f2(a, b)), la, lb);
+  a = fabsf(a * x) <= 0.25f ? la : soft_cap(a, in, out);
+  b = fabsf(b * x) <= 0.25f ? lb : soft_cap(b, in, out);
+}
 
 __device__ __forceinline__ void cluster_barrier() {
   asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
@@ -127,7 +136,7 @@ struct Joined {
   float m = -INFINITY, l = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
   __device__ __forceinline__ void add(float pm, float pl, const float4& po) {
-    if (pm == -CUDART_INF_F) return;                        // a piece without keys
+    if (pl == 0.f) return;                                  // a piece without keys
     const float top = fmaxf(m, pm);
     const float a = m == -CUDART_INF_F ? 0.f : fast_exp2(m - top), b = fast_exp2(pm - top);
     m = top;
@@ -139,10 +148,10 @@ struct Joined {
   }
 };
 
-// Columns d .. d + 3 of an output row of dv, rounded once; a row that saw no key is zero.
+// Columns d .. d + 3 of an output row of dv, rounded once; a row that saw no key is zero (a sum that is no number stays one).
 template <typename T> __device__ __forceinline__ void store_joined(T* out_row, int d, int dv, const Joined& j) {
   if (d >= dv) return;
-  const float inv = j.l > 0.f ? 1.f / j.l : 0.f;
+  const float inv = j.l == 0.f ? 0.f : 1.f / j.l;
   typename Elem<T>::T2 v[2] = {Elem<T>::from_f2(j.o.x * inv, j.o.y * inv), Elem<T>::from_f2(j.o.z * inv, j.o.w * inv)};
   *reinterpret_cast<uint2*>(out_row + d) = *reinterpret_cast<const uint2*>(v);
 }

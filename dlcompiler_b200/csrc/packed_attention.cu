@@ -21,6 +21,7 @@
 // O += P_{j-1} V_{j-1} with P as the A operand from TMEM), warps 0-3 the softmax, one thread per row.  The blocks of
 // 64 keys are those of the sinks and then those of the window; blocks in between are skipped, and so are pages
 // that hold no key which the tile sees.
+#include <float.h>
 #include <math_constants.h>
 
 #include "cluster_decode.cuh"
@@ -426,9 +427,9 @@ packed_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
         };
         float mx = 0.f;
         if (CAP) {
-          // Scores below the cap, which they nearly always are, go through a polynomial, a short one below a quarter of it: the exponential and the reciprocal of the
-          // other way take the special-function unit twice as long as the softmax itself.  Keys out of sight count as 0 so far:
-          // what was not fetched is anything.
+          // Scores below the cap, which they nearly always are, go through a polynomial, a short one below a quarter of it: the
+          // exponential and the reciprocal of the other way take the special-function unit twice as long as the softmax itself
+          // (chunks of 24 sequences 171 -> 139 -> 131 us).  Keys out of sight count as 0 so far: what was not fetched is anything.
           if (!whole) hide(0u);
           float m4[4] = {CUDART_INF_F, CUDART_INF_F, CUDART_INF_F, CUDART_INF_F};
 #pragma unroll
@@ -443,6 +444,8 @@ packed_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
           mx = largest();
           const float size = fmaxf(mx, -fminf(min3(m4[0], m4[1], m4[2]), m4[3]));
           auto each_pair = [&](auto&& f) {
+            float unused;
+            unpack_f2(f(pack_f2(mx, mx)), mx, unused);
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -453,18 +456,20 @@ packed_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
                 sr[h][c + 1] = __float_as_uint(b);
               }
           };
-          if (cap_x <= 1e8f && !__any_sync(0xffffffffu, live && !(size * cap_x <= 0.25f))) {     // x^4 is a number
-            each_pair(SoftCapShort(cap_x, p.scale_log2));
+          const SoftCapShort cap_short(cap_x, p.scale_log2);
+          if (!__any_sync(0xffffffffu, live && !(size * cap_x <= 0.25f))) {
+            each_pair(cap_short);
           } else if (!__any_sync(0xffffffffu, live && !(size * cap_x <= 1.f))) {
             const uint64_t x2 = pack_f2(cap_x, cap_x), out2 = pack_f2(p.scale_log2, p.scale_log2);
             each_pair([&](uint64_t v) { return soft_cap_below(v, x2, out2); });
           } else {
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-              for (int c = 0; c < 32; ++c) sr[h][c] = __float_as_uint(soft_cap(__uint_as_float(sr[h][c]), cap_in, cap_out));
+            each_pair([&](uint64_t v) {
+              float a, b;
+              unpack_f2(v, a, b);
+              soft_cap_any(a, b, cap_short, cap_x, cap_in, cap_out);
+              return pack_f2(a, b);
+            });
           }
-          mx = soft_cap(mx, cap_in, cap_out);
         }
         if (!whole) hide(0xff800000u);                // -inf
         // p = 2^(s * scale - m) as 16-bit pairs, and their sum
@@ -559,7 +564,7 @@ packed_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
       // O in 32 bits over Q and K (every MMA has retired), 16-byte chunk q of row r at q ^ (r & 7); maximum and sum over V
       float* ml = reinterpret_cast<float*>(smem + OFF_V);
       ml[row] = ok ? m_ref : -CUDART_INF_F;
-      ml[BM + row] = l_sum;
+      ml[BM + row] = ok ? l_sum : 0.f;
 #pragma unroll 1
       for (int c = 0; ok && busy && nb > 0 && c < D / 32; ++c) {
         uint32_t o[32];
@@ -573,7 +578,7 @@ packed_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
     } else if (ok) {
       // Through the Q tile's shared memory (every Q K^T has retired; row r of O over row r of Q, same swizzle), 64
       // columns at a time, so that the lanes of a store cover whole 128-byte lines.  A row that saw no key is zero.
-      const float inv_l = l_sum > 0.f ? 1.f / l_sum : 0.f;
+      const float inv_l = 1.f / l_sum;
       uint8_t* stage = smem + OFF_Q;
       const int sub = lane >> 3, cc = lane & 7;              // row of four, 16-byte chunk of its line
       T* obase = reinterpret_cast<T*>(p.out) + (int64_t)(start + q0) * p.o_st + (int64_t)kvh * p.group * p.o_sh + cc * 8;
@@ -592,7 +597,7 @@ packed_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
           for (int u = 0; u < 4; ++u) {
             const int e = (v & 3) * 8 + 2 * u;
             typename Elem<T>::T2 v2 = Elem<T>::from_f2(__uint_as_float(o[v >> 2][e]) * inv_l, __uint_as_float(o[v >> 2][e + 1]) * inv_l);
-            w[u] = l_sum > 0.f ? *reinterpret_cast<uint32_t*>(&v2) : 0u;
+            w[u] = l_sum == 0.f ? 0u : *reinterpret_cast<uint32_t*>(&v2);
           }
           *reinterpret_cast<uint4*>(stage + c * Q_BOX + row * 128 + ((v ^ (row & 7)) << 4)) =
               make_uint4(w[0], w[1], w[2], w[3]);
@@ -687,7 +692,7 @@ static int launch_packed(const CUtensorMap& tq, const CUtensorMap& tk, const CUt
 // What both entry points take: types, head sizes, cache layout.  Returns DLB_OK or an error; `width` is the tile width.
 static int check_attention(const char* what, int64_t batch, int64_t tokens, int64_t hq, int64_t hkv, int64_t head_dim,
                            int64_t head_dim_v, int64_t page_size, int64_t num_pages, int64_t max_pages, float sm_scale,
-                           int dtype, int& width) {
+                           float& softcap, int dtype, int& width) {
   DLB_CHECK_ARG(dtype == DLB_DTYPE_BF16 || dtype == DLB_DTYPE_F16, DLB_ERR_UNSUPPORTED, "%s: dtype %d (need fp16 or bf16)",
                 what, dtype);
   DLB_CHECK_ARG(head_dim >= 8 && head_dim <= 128 && head_dim % 8 == 0 && head_dim_v >= 8 && head_dim_v <= 128 &&
@@ -703,8 +708,10 @@ static int check_attention(const char* what, int64_t batch, int64_t tokens, int6
   DLB_CHECK_ARG(num_pages < (1LL << 31) && max_pages * page_size < (1LL << 31) && tokens * hq < (1LL << 31) &&
                     batch <= 65535 && hkv * ((hq / hkv + 15) / 16) <= 65535,
                 DLB_ERR_TOO_LARGE, "%s: sizes past 31 bits", what);
+  if (softcap > FLT_MAX) softcap = 0.f;       // as good as none
   // the maximum is taken before the scale is applied
   DLB_CHECK_ARG(sm_scale > 0.f, DLB_ERR_BAD_ARG, "%s: sm_scale must be positive", what);
+  DLB_CHECK_ARG(!(softcap > 0.f) || sm_scale / softcap <= 1e8f, DLB_ERR_UNSUPPORTED, "%s: soft-cap %g too small", what, (double)softcap);
   width = (head_dim <= 64 && head_dim_v <= 64) ? 64 : 128;
   return DLB_OK;
 }
@@ -772,7 +779,7 @@ extern "C" int dlb_sink_attention(const void* q, const void* k_cache, const void
   using namespace dlb;
   int width = 0;
   int rc = check_attention("sink_attention", batch, total_q_tokens, hq, hkv, head_dim, head_dim_v, page_size, num_pages,
-                           max_pages, sm_scale, dtype, width);
+                           max_pages, sm_scale, softcap, dtype, width);
   if (rc != DLB_OK) return rc;
   DLB_CHECK_ARG(window >= 0 && sinks >= 0 && max_q_len >= 0, DLB_ERR_BAD_ARG, "sink_attention: negative window, sinks or length");
   if (batch == 0 || total_q_tokens == 0 || max_q_len == 0) return DLB_OK;
@@ -841,7 +848,7 @@ extern "C" int dlb_shared_prefix_attention(
   using namespace dlb;
   int width = 0;
   int rc = check_attention("shared_prefix_attention", batch, batch, hq, hkv, head_dim, head_dim_v, page_size, num_pages,
-                           max_pages < prefix_max_pages ? max_pages : prefix_max_pages, sm_scale, dtype, width);
+                           max_pages < prefix_max_pages ? max_pages : prefix_max_pages, sm_scale, softcap, dtype, width);
   if (rc != DLB_OK) return rc;
   DLB_CHECK_ARG(groups >= 1 && groups <= 65535 && prefix_max_pages * page_size < (1LL << 31) &&
                     max_pages * page_size < (1LL << 31),

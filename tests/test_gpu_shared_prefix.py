@@ -206,3 +206,20 @@ def test_large_scores(cuda_device):
     b.q *= 12
     b.check(b.run())
     b.check(b.run(cap=20.0), cap=20.0)                       # scores on both sides of the cap
+
+
+@pytest.mark.parametrize("cap", [None, 20.0, float("inf")])
+def test_no_numbers_in_visible_places(cuda_device, cap):
+    """Heads of q that are no number, a key of a prefix and one of a sequence: their rows of the output are none either, and no
+    other."""
+    b = Groups(cuda_device, [7, 5], [700, 65], list(range(12)), poison=False)
+    ref = b.run(cap=cap).clone()
+    b.q[2, 3, 1] = b.q[11, 0, 0] = float("nan")
+    b.k.view(-1, 2, 64)[rows_of(b.prefix_table[1], 65, 16)[64], 1] = float("nan")
+    b.k.view(-1, 2, 64)[rows_of(b.table[4], 4, 16)[0], 0] = float("nan")
+    lost = torch.zeros(12, 8, dtype=torch.bool, device=cuda_device)
+    lost[2, 3] = lost[11, 0] = lost[4, :4] = lost[7:, 4:] = True
+    o = b.run(cap=cap, o=torch.empty_like(b.o))
+    assert o[lost].isnan().all() and not o[~lost].isnan().any()
+    # two results of the same scores, each off by a rounding of P and one of the output
+    assert (o[~lost].float() - ref[~lost].float()).abs().max() <= 2 * 2 * 2 ** -8 * b.v.abs().max()

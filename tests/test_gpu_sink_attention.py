@@ -273,6 +273,44 @@ def test_large_scores_and_infinite_values_behind_the_window(cuda_device):
         b.check(b.run(cap=20.0), cap=20.0)                   # scores on both sides of the cap
 
 
+@pytest.mark.parametrize("new", [[1, 1, 1], [70, 3, 20]])
+@pytest.mark.parametrize("cap", [1e6, 1e30, float("inf")])
+def test_cap_far_above_the_scores(cuda_device, new, cap):
+    """Takes off x^2 / 3 of a score, x its size over the cap: nothing here (10^-10 of it at most)."""
+    b = Batch(cuda_device, new, [500, 30, 1], 150, 5)
+    b.check(b.run(cap=cap))
+
+
+@pytest.mark.parametrize("new", [[1, 1, 1], [70, 3, 20]])
+@pytest.mark.parametrize("cap", [0.0, 30.0])
+def test_no_numbers_in_visible_places(cuda_device, new, cap):
+    """A head of q that is no number: its row of the output is none either, the others are as without it.  A key that is no
+    number: so are the queries that see it, and no other."""
+    b = Batch(cuda_device, new, [500, 30, 1], 150, 5, poison=False)
+    q = b.q.clone()
+    for t, h in ((0, 0), (0, 5), (sum(new) - 1, 7)):
+        q[t, h, 3] = float("nan")
+    o = b.run(cap=cap or None, q=q)
+    lost = q.isnan().any(-1)
+    assert o[lost].isnan().all()
+    o[lost] = b.run(cap=cap or None, o=torch.empty_like(b.o))[lost]
+    b.check(o, cap=cap)
+
+    whole = b.run(cap=cap or None, o=torch.empty_like(b.o))
+    at = 0
+    for s, past in enumerate(b.past):
+        b.k.view(-1, 2, 64)[rows_of(b.clean[s], past + 1, 16)[-1], 1] = float("nan")      # the first new token
+    o = b.run(cap=cap or None)
+    for s, (n, past) in enumerate(zip(new, b.past)):
+        sees = b.seen(s, cuda_device)[:, past]
+        assert sees[0] and o[at:at + n][sees, 4:].isnan().all()
+        assert not o[at:at + n, :4].isnan().any() and not o[at:at + n][~sees].isnan().any()
+        at += n
+    keep = ~o.isnan()
+    # two results of the same scores, each off by a rounding of P and one of the output
+    assert (o[keep].float() - whole[keep].float()).abs().max() <= 2 * 2 * 2 ** -8 * b.v.abs().max()
+
+
 def test_empty_calls(cuda_device):
     b = Batch(cuda_device, [2], [10], 5, 1)
     e = b.q[:0]

@@ -120,29 +120,29 @@ def test_attention_entries():
     lib = _lib.load()
 
     def sink(q=16, tokens=3, batch=3, most=1, hq=4, hkv=2, d=64, dv=64, page=16, pages=4, cols=2, q_st=256, o_sh=64,
-             window=8, sinks=2, scale=0.1, dtype=_lib.DTYPE_BF16):
+             window=8, sinks=2, scale=0.1, cap=-1.0, dtype=_lib.DTYPE_BF16):
         return lib.dlb_sink_attention(q, 16, 16, 16, 16, 16, 16, 16, batch, tokens, most, hq, hkv, d, dv, page, pages, cols,
                                       q_st, 64, 256, o_sh, 2048, 128, 64, 2048, 128, 64, 2, 0, 0, 0, 0, window, sinks, scale,
-                                      -1.0, dtype, None, None)
+                                      cap, dtype, None, None)
 
     for bad in (dict(q=None), dict(q=8), dict(tokens=-1), dict(hq=3), dict(hq=258, hkv=2), dict(d=12), dict(d=136),
                 dict(dv=0), dict(page=24), dict(page=8), dict(pages=0), dict(cols=0), dict(q_st=252), dict(o_sh=4),
-                dict(window=-1), dict(sinks=-1), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")),
+                dict(window=-1), dict(sinks=-1), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(cap=1e-30),
                 dict(dtype=_lib.DTYPE_F32), dict(batch=70000), dict(cols=1 << 28), dict(most=-1)):
         assert sink(**bad) < 0 and lib.dlb_last_error().startswith(b"sink_attention"), bad
     for nothing in (dict(batch=0), dict(tokens=0), dict(most=0)):
         assert sink(**nothing) == 0
 
     def prefix(q=16, partial=16, batch=3, groups=2, hq=4, hkv=2, d=64, page=16, prefix_cols=2, cols=2, chunk=64, cluster=1,
-               scale=0.1, dtype=_lib.DTYPE_BF16):
+               scale=0.1, cap=-1.0, dtype=_lib.DTYPE_BF16):
         return lib.dlb_shared_prefix_attention(q, 16, 16, 16, 16, 16, 16, 16, 16, partial, batch, groups, hq, hkv, d, 64,
                                                page, 4, prefix_cols, cols, 256, 64, 256, 64, 2048, 128, 64, 2048, 128, 64,
-                                               2, 2, 0, 0, 0, 0, 0, chunk, cluster, scale, -1.0, dtype, None, None)
+                                               2, 2, 0, 0, 0, 0, 0, chunk, cluster, scale, cap, dtype, None, None)
 
     for bad in (dict(q=None), dict(partial=None), dict(partial=8), dict(batch=-1), dict(groups=0), dict(groups=80000),
                 dict(hq=3), dict(d=12), dict(page=8), dict(prefix_cols=0), dict(cols=0), dict(chunk=0), dict(chunk=100),
                 dict(cluster=0), dict(cluster=3), dict(cluster=16),
-                dict(scale=0.0), dict(dtype=_lib.DTYPE_F32), dict(prefix_cols=1 << 28), dict(cols=1 << 28)):
+                dict(scale=0.0), dict(cap=1e-30), dict(dtype=_lib.DTYPE_F32), dict(prefix_cols=1 << 28), dict(cols=1 << 28)):
         assert prefix(**bad) < 0 and lib.dlb_last_error().startswith(b"shared_prefix_attention"), bad
     assert prefix(batch=0) == 0
     assert lib.dlb_shared_prefix_workspace_floats(3, 4, 96, 5) == 3 * 4 * 5 * 130
