@@ -374,6 +374,9 @@ packed_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
     // A warp whose rows are all past the tile's last one keeps in step and computes nothing: its P and O stay what they are, and
     // no other row reads them.
     const bool busy = warp * 32 < tile_rows;
+    // what every row of the warp sees, but for the sinks
+    const int whole_to = min(keys, hist + q0 + (int)((uint32_t)(warp * 32) * p.group_inv >> 16) + 1);
+    const int whole_from = hist + q0 + (int)((uint32_t)(max(min(warp * 32 + 32, tile_rows), 1) - 1) * p.group_inv >> 16) - p.window;
     for (int j = 0; j < nb; ++j) {
       const int s = j % STAGES;
       ok = mbar_wait(&qk_done[s], (j / STAGES) & 1, abort_flag, p.status, 58, j);
@@ -382,9 +385,8 @@ packed_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
       tc_fence_after_sync();
       const uint32_t s_cols = tmem_base + lane_field + (j & 1) * BN;
       const int key0 = block_key(j);
-      // blocks that some row sees only in part
-      const bool whole = MODE == PREFILL ? key0 + BN - 1 <= hist + q0 && key0 + BN <= keys && key0 >= pos_hi - p.window
-                                         : key0 + BN <= keys;
+      // does every row of the warp see the whole block?
+      const bool whole = MODE == PREFILL ? key0 + BN <= whole_to && (key0 >= whole_from || key0 + BN <= p.sinks) : key0 + BN <= keys;
       if (busy) {
         uint32_t sr[2][32];
         tmem_ld_32x32b_x32(s_cols, sr[0]);
@@ -429,8 +431,7 @@ packed_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
         if (CAP) {
           // Scores below the cap, which they nearly always are, go through a polynomial, a short one below a quarter of it: the
           // exponential and the reciprocal of the other way take the special-function unit twice as long as the softmax itself
-          // (chunks of 24 sequences 171 -> 139 -> 131 us).  Keys out of sight count as 0 so far: what was not fetched is anything.
-          if (!whole) hide(0u);
+          // (chunks of 7 prompts 157 -> 139 -> 131 us).  Keys out of sight are anything here, and may lead the longer way.
           float m4[4] = {CUDART_INF_F, CUDART_INF_F, CUDART_INF_F, CUDART_INF_F};
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
@@ -536,20 +537,21 @@ packed_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
         tmem_st_32x32b_x16(s_cols, pk[0]);
         tmem_st_32x32b_x16(s_cols + 16, pk[1]);
       }
-      if (!whole && !(key0 >= vis_lo && key0 + BN <= vis_hi)) {
+      if (!whole && !(key0 >= vis_lo && key0 + BN <= vis_hi) && !(MODE == PREFILL && key0 + BN <= min(p.sinks, vis_hi))) {
         // V rows that no row of the tile sees (past the end, behind the window of every row, not fetched): their weights
         // are zero, but 0 x (what a reused page or an old tile left there) may be NaN.  Zeroed, and made visible to the
-        // tensor core's reads, before this block's P V can be issued.
-        ok = mbar_wait(&v_full[s], (j / STAGES) & 1, abort_flag, p.status, 61, j);
+        // tensor core's reads, before this block's P V can be issued.  Two threads to a row.
+        const int r = threadIdx.x >> 1;
+        if (!seen(key0 + r, key0 + r + 1)) {
+          ok = mbar_wait(&v_full[s], (j / STAGES) & 1, abort_flag, p.status, 61, j);
+          uint8_t* vt = smem + OFF_V + s * KV_BYTES + r * 128;
+#pragma unroll
+          for (int u = 0; u < BOXES * 4; ++u)
+            *reinterpret_cast<uint4*>(vt + (u >> 2) * KV_BOX + (((threadIdx.x & 1) * 4 + (u & 3) + r) & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+          fence_proxy_async_smem();
+        }
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        uint8_t* vt = smem + OFF_V + s * KV_BYTES;
-        for (int u = threadIdx.x; u < BN * BOXES * 8; u += 128) {
-          const int chunk = u & 7, bx = (u >> 3) % BOXES, r = (u >> 3) / BOXES;
-          if (!seen(key0 + r, key0 + r + 1))
-            *reinterpret_cast<uint4*>(vt + bx * KV_BOX + r * 128 + chunk * 16) = make_uint4(0u, 0u, 0u, 0u);
-        }
-        fence_proxy_async_smem();
       }
       tmem_wait_st();
       tc_fence_before_sync();
