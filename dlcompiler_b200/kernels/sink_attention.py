@@ -74,14 +74,16 @@ def sink_attention_fwd(
     [num_pages, page_size, Hkv, D], which already hold the new tokens, `o` [total_q, Hq, Dv] written in place,
     `block_offsets` [batch, max_pages], `kv_seqlens` [batch] tokens in the cache, the new ones included; index tensors
     int32 or int64.  `max_seqlen` is the largest of `q_seqlens`: 1 takes the form for single tokens (sequences with
-    none are left out), anything larger the one for chunks of prompts or several drafted tokens, any mixture of
-    lengths.  Rows of `q` and `o` that belong to no sequence are left as they are; a query that sees no key gets zeros.
+    none are left out, of longer ones only the first token is computed), anything larger the one for chunks of prompts or
+    several drafted tokens, any mixture of lengths.  Rows of `q` and `o` that belong to no sequence are left as they are; a
+    query that sees no key gets zeros.
 
     Only pages with a token that some query of a tile of 128 rows sees are looked at: entries of `block_offsets` for
     tokens behind the window may be stale.  A page outside the cache where a visible token should be is an error
     (`check_device_status()` raises), and its sequence's output is undefined.  fp16/bf16, head sizes multiples of 8 up
     to 128, page size a power of two >= 16, at most 128 query heads to a key head, `o` and the caches 16-byte aligned
-    in their rows.
+    in their rows, `sm_scale` positive.  An infinity or NaN in a visible token's values reaches every query of the sequence
+    that shares a tile with one that sees it (its weight there is 0, and 0 x inf is no number).
     """
     dev = _lib.require_cuda(q, k, v, o, block_offsets, q_start_loc, q_seqlens, kv_seqlens)
     q, (tokens, hq, hkv, dk, dv, page, pages), strides = check_paged(q, k, v, o)
@@ -97,7 +99,8 @@ def sink_attention_fwd(
         rc = lib.dlb_sink_attention(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), block_offsets.data_ptr(), q_start_loc.data_ptr(),
             q_seqlens.data_ptr(), kv_seqlens.data_ptr(), batch, tokens, int(max_seqlen), hq, hkv, dk, dv, page, pages,
-            columns, *strides, bt_stride, *wide, min(int(window_size), 2**31), min(int(num_sinks), 2**31), dk ** -0.5 if sm_scale is None else sm_scale,
-            logit_softcapping or -1.0, _lib.dtype_code(q), _lib.status_word(dev).data_ptr(), _lib.stream_ptr(dev))
+            columns, *strides, bt_stride, *wide, min(int(window_size), 2**31), min(int(num_sinks), 2**31),
+            dk ** -0.5 if sm_scale is None else sm_scale, logit_softcapping or -1.0, _lib.dtype_code(q),
+            _lib.status_word(dev).data_ptr(), _lib.stream_ptr(dev))
     _lib.check(rc, "sink_attention_fwd")
     return o

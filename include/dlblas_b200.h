@@ -295,8 +295,8 @@ int dlb_paged_decode_rows(const void* q, const void* k_cache, const void* v_cach
  * hold the new tokens, block_table [batch, max_pages], kv_seq_len [batch] with the new tokens; every index array int32
  * or int64.  max_q_len is the largest of q_seq_len; 1 selects the form for single tokens.  Rows of no sequence are not
  * written, queries without a key get zeros, pages without a visible token are not looked at.  softcap > 0: scores become
- * softcap * tanh(score * sm_scale / softcap).  hq / hkv <= 128, head sizes multiples of 8 up to 128, fp16 / bf16,
- * sm_scale > 0, rows of q, out and the caches 16-byte aligned.  The reference has the window without sinks
+ * softcap * tanh(score * sm_scale / softcap), softcap >= 1e-8 sm_scale.  hq / hkv <= 128, head sizes multiples of 8 up
+ * to 128, fp16 / bf16, sm_scale > 0, rows of q, out and the caches 16-byte aligned.  The reference has the window without sinks
  * (python/dlBLAS/dlblas/kernels/paged_attention.py:421-424, 447). */
 int dlb_sink_attention(const void* q, const void* k_cache, const void* v_cache, void* out, const void* block_table,
                        const void* q_start_loc, const void* q_seq_len, const void* kv_seq_len, int64_t batch,
@@ -312,10 +312,10 @@ int dlb_sink_attention(const void* q, const void* k_cache, const void* v_cache, 
  * prefix of its group, then its own tokens.  q [batch, hq, head_dim], out [batch, hq, head_dim_v]; group g is the
  * sequences group_start[g] .. group_start[g + 1] - 1 (group_start [groups + 1]), its prefix the first prefix_len[g] tokens
  * of row g of prefix_table [groups, prefix_max_pages]; a sequence's own tokens are the first kv_seq_len[b] of row b of
- * block_table [batch, max_pages].  `chunk` (a multiple of 64) tokens of a prefix go to a split, which `cluster` (1, 2, 4 or 8) CTAs share; `partial` is a workspace
- * of dlb_shared_prefix_workspace_floats(batch, hq, larger head size, ceil(prefix_max_pages * page_size / chunk)) fp32,
- * 16-byte aligned, in use until the call's work on the stream is done.  Two launches.  Everything else as for
- * dlb_sink_attention.  No counterpart in the reference. */
+ * block_table [batch, max_pages].  `chunk` (a multiple of 64) tokens of a prefix go to a split, which `cluster` (1, 2, 4
+ * or 8) CTAs share; `partial` is a workspace of dlb_shared_prefix_workspace_floats(batch, hq, larger head size,
+ * ceil(prefix_max_pages * page_size / chunk)) fp32, 16-byte aligned, in use until the call's work on the stream is done.
+ * Two launches.  Everything else as for dlb_sink_attention.  No counterpart in the reference. */
 int64_t dlb_shared_prefix_workspace_floats(int64_t tokens, int64_t hq, int64_t head_dim, int64_t splits);
 int dlb_shared_prefix_attention(const void* q, const void* k_cache, const void* v_cache, void* out,
                                 const void* prefix_table, const void* prefix_len, const void* group_start,
