@@ -82,10 +82,10 @@ cluster_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
   // ---- the sequence: its row of q, its keys ----
   const int page_size = 1 << p.page_shift;
   int64_t row = b;
-  int ctx = load_index(p.kv_lens, b, p.lens_is_int64);
+  int ctx = clamped_index(p.kv_lens, b, p.lens_is_int64);
   if (!PREFIX) {
-    const int q_len = load_index(p.q_lens, b, p.qlens_is_int64);
-    row = load_index(p.q_start, b, p.start_is_int64);
+    const int q_len = clamped_index(p.q_lens, b, p.qlens_is_int64);
+    row = clamped_index(p.q_start, b, p.start_is_int64);
     if (q_len <= 0 || row < 0 || row >= p.tokens) return;    // the whole cluster leaves
     ctx -= q_len - 1;                                        // its first token (there is one)
   }
@@ -155,7 +155,7 @@ cluster_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
     auto entry = [&](int t) {
       bool wanted;
       const int64_t column = lane_token(t, wanted) >> p.page_shift;
-      return wanted ? load_index(p.block_table, (int64_t)b * p.bt_stride + column, p.table_is_int64) : 0;
+      return wanted ? clamped_index(p.block_table, (int64_t)b * p.bt_stride + column, p.table_is_int64) : 0;
     };
     int pages = 0, pages_next = entry(t_lo);
     for (int t = t_lo; t < t_hi; ++t) {
@@ -228,7 +228,7 @@ cluster_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
         if (g0 + lane < p.prefix.groups) group_rows(p.prefix, p.tokens, g0 + lane, start, rows);
         const uint32_t has = __ballot_sync(0xffffffffu, b >= start && b < start + rows);
         if (has != 0) {
-          n = prefix_splits(p.prefix, load_index(p.prefix.lens, g0 + __ffs(has) - 1, p.prefix.lens_is_int64));
+          n = prefix_splits(p.prefix, clamped_index(p.prefix.lens, g0 + __ffs(has) - 1, p.prefix.lens_is_int64));
           break;
         }
       }

@@ -1,5 +1,6 @@
 // Single-token attention split over a thread-block cluster (cluster_decode.cu), as its callers see it.
 #pragma once
+#include <limits.h>
 #include <math_constants.h>
 
 #include <atomic>
@@ -46,6 +47,12 @@ struct ClusterDecodeParams {
   int* status;
   PrefixPartials prefix;       // o == null: none
 };
+
+// Entry i of an index array; 64-bit ones are kept inside 32 bits, where a page, a row or a length out there stays out of range.
+__device__ __forceinline__ int clamped_index(const void* p, int64_t i, int is64) {
+  if (!is64) return reinterpret_cast<const int32_t*>(p)[i];
+  return (int)max((int64_t)INT_MIN, min((int64_t)INT_MAX, reinterpret_cast<const int64_t*>(p)[i]));
+}
 
 // Records a page that does not exist where a visible token should be.
 __device__ __forceinline__ void report_bad_page(int* status, int row, int column, int page) {

@@ -90,11 +90,11 @@ template <int MODE>
 __device__ __forceinline__ void packed_rows(const PackedParams& p, int b, int& start, int& n, int& kv_len) {
   if (MODE == pa::PREFIX) {
     group_rows(p.prefix, p.tokens, b, start, n);
-    kv_len = load_index(p.prefix.lens, b, p.prefix.lens_is_int64);
+    kv_len = clamped_index(p.prefix.lens, b, p.prefix.lens_is_int64);
   } else {
-    start = load_index(p.q_start, b, p.start_is_int64);
-    n = load_index(p.q_lens, b, p.qlens_is_int64);
-    kv_len = load_index(p.kv_lens, b, p.lens_is_int64);
+    start = clamped_index(p.q_start, b, p.start_is_int64);
+    n = clamped_index(p.q_lens, b, p.qlens_is_int64);
+    kv_len = clamped_index(p.kv_lens, b, p.lens_is_int64);
     n = (start < 0 || start >= p.tokens) ? 0 : (int)min((int64_t)max(n, 0), p.tokens - start);
   }
 }
@@ -181,7 +181,7 @@ packed_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
     return;
   const int q0 = tile * p.tile_tokens;
   const int tile_rows = min(p.tile_tokens, n - q0) * p.group;        // rows of this tile that exist
-  const int hist = kv_len - (MODE == PREFILL ? load_index(p.q_lens, seq, p.qlens_is_int64) : 0);
+  const int hist = kv_len - (MODE == PREFILL ? clamped_index(p.q_lens, seq, p.qlens_is_int64) : 0);
   const int keys = (int)max((int64_t)0, min((int64_t)kv_len, (int64_t)p.max_pages << p.page_shift));
   // positions of the tile's first and last token; the keys that some row sees are [vis_lo, vis_hi) and those below sinks
   int vis_lo = 0, vis_hi = keys, pos_hi = 0, sink_blocks = 0, first_block, nb;
@@ -280,7 +280,8 @@ packed_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
         return j + (lane >> boxes_shift) < nb && seen(lane_key(j), lane_key(j) + (1 << box_shift));
       };
       auto entry = [&](int j) {
-        return wanted(j) ? load_index(p.block_table, (int64_t)seq * p.bt_stride + (lane_key(j) >> p.page_shift), p.table_is_int64) : 0;
+        return wanted(j) ? clamped_index(p.block_table, (int64_t)seq * p.bt_stride + (lane_key(j) >> p.page_shift), p.table_is_int64)
+                         : 0;
       };
       int pages = 0, pages_next = entry(0);
       for (int j = 0; j < nb; ++j) {

@@ -225,6 +225,33 @@ def test_page_outside_the_cache(cuda_device, most):
         b.table = table
 
 
+@pytest.mark.parametrize("most", [1, 3])
+def test_64_bit_indices_past_32_bits(cuda_device, most):
+    """A page 2^32 is not page 0, nor a row or a length of that size one of 0."""
+    b = Batch(cuda_device, [most] * 3, [100, 120, 140], 64, 4, idx=torch.int64, poison=False)
+    ref = b.run().clone()
+    b.table[1, 6] = 2 ** 32
+    b.run(o=torch.empty_like(b.o))
+    with pytest.raises(DlblasError, match=f"row 1, column 6 .* page {2 ** 31 - 1},"):
+        check_device_status()
+    b.table[1, 6] = -2 ** 32
+    b.run(o=torch.empty_like(b.o))
+    with pytest.raises(DlblasError, match=f"row 1, column 6 .* page {-2 ** 31},"):
+        check_device_status()
+    b.table = b.clean
+    for far in (2 ** 32, 2 ** 32 + most, -2 ** 32):
+        start = b.start
+        b.start = start.clone()
+        b.start[1] = far
+        o = b.run(o=torch.full_like(b.o, 7.0))
+        assert (o[most:2 * most] == 7).all() and torch.equal(o[:most], ref[:most]) and torch.equal(o[2 * most:], ref[2 * most:])
+        b.start = start
+    b.kv = b.kv.clone()
+    b.kv[1] = -2 ** 32 + 100
+    assert not b.run(o=torch.empty_like(b.o))[most:2 * most].any()
+    check_device_status()
+
+
 @pytest.mark.parametrize("most", [1, 40])
 def test_graph_streams_and_repeats(cuda_device, most):
     """The same bits every time, on another stream, and from a graph replayed with other lengths."""
