@@ -78,6 +78,12 @@ cluster_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
   const int b = blockIdx.z;
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
+  if (warp == CONSUMERS && lane == 0) {
+    tma_prefetch_desc(&tmap_k);
+    tma_prefetch_desc(&tmap_v);
+    tma_prefetch_desc(&edge_k);
+    tma_prefetch_desc(&edge_v);
+  }
 
   // ---- the sequence: its row of q, its keys ----
   const int page_size = 1 << p.page_shift;
@@ -134,12 +140,6 @@ cluster_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
 
   if (warp == CONSUMERS) {
     // ------------------------------ producer ------------------------------
-    if (lane == 0) {
-      tma_prefetch_desc(&tmap_k);
-      tma_prefetch_desc(&tmap_v);
-      tma_prefetch_desc(&edge_k);
-      tma_prefetch_desc(&edge_v);
-    }
     // One table entry per lane: `units` pages (or pieces of 64 slots) to a tile, 32 / units tiles to a batch.  The next batch's
     // entries are asked for when this one's come into use, and looked at only then.
     const int unit_shift = min(p.page_shift, 6);

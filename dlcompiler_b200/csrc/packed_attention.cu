@@ -162,6 +162,11 @@ packed_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
   constexpr int OFF_Q = L::OFF_Q, OFF_K = L::OFF_K, OFF_V = L::OFF_V, OFF_CTRL = L::OFF_CTRL;
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
+  if (warp == WARP_TMA && lane == 0) {
+    tma_prefetch_desc(&tmap_q);
+    tma_prefetch_desc(&tmap_k);
+    tma_prefetch_desc(&tmap_v);
+  }
   // ---- which tile: PREFILL has the kv heads of a tile side by side, PREFIX the row tiles of a (kv head, split), which
   // read the same keys; the CTAs of a cluster share one ----
   const int cluster = p.cluster, rank = (int)blockIdx.x & (cluster - 1);
@@ -245,10 +250,16 @@ packed_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
     tmem_alloc(tmem_slot, TMEM_COLS);
     tmem_relinquish();
   }
-  tc_fence_before_sync();
-  __syncthreads();
-  tc_fence_after_sync();
-  const uint32_t tmem_base = *tmem_slot;
+  // The loading warp, which set up the barriers, needs nothing of the others and does not wait for them (and the tensor memory)
+  if (warp == WARP_TMA) {
+    __syncwarp();
+    asm volatile("bar.arrive 1, %0;" ::"n"(THREADS) : "memory");
+  } else {
+    tc_fence_before_sync();
+    asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory");
+    tc_fence_after_sync();
+  }
+  const uint32_t tmem_base = warp == WARP_TMA ? 0u : *tmem_slot;
   const uint32_t tmem_o = tmem_base + 128;
 
   float m_ref = -CUDART_INF_F;                     // softmax warps: reference maximum (scaled, base-2 domain) and sum
@@ -263,9 +274,6 @@ packed_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
     // scheduler with two busy softmax warps, so an instruction takes it about ten clocks, and a late load holds up everything.
     if (nb > 0) {
       if (lane == 0) {
-        tma_prefetch_desc(&tmap_q);
-        tma_prefetch_desc(&tmap_k);
-        tma_prefetch_desc(&tmap_v);
         mbar_arrive_expect_tx(q_full, BOXES * p.group * p.tile_tokens * 128);
 #pragma unroll
         for (int bx = 0; bx < BOXES; ++bx)
