@@ -262,8 +262,7 @@ packed_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
   const uint32_t tmem_base = warp == WARP_TMA ? 0u : *tmem_slot;
   const uint32_t tmem_o = tmem_base + 128;
 
-  float m_ref = -CUDART_INF_F;                     // softmax warps: reference maximum (scaled, base-2 domain) and sum
-  float l_sum = 0.f;
+  float m_ref = 0.f, l_sum = 0.f;                  // softmax warps: reference maximum (scaled, base-2 domain) and sum
   const int row = threadIdx.x;                     // row of the tile == TMEM lane
   const uint32_t lane_field = (uint32_t)(warp * 32) << 16;
 
@@ -520,16 +519,22 @@ packed_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
           unpack_f2(add_f2(sum2a, sum2b), a, b);
           return a + b;
         };
-        // With the reference maximum as it is, which nearly always stays: so the exponentials do not wait for this block's maximum
+        // With the reference as it is, which nearly always stays: so the exponentials do not wait for this block's maximum
         float sum = weigh(m_ref);
         if (!CAP || !whole) mx = largest() * eff_scale;
         if (!live) mx = -CUDART_INF_F;                  // rows past the tile's last token never ask for more
-        // also a row's first visible key: m_ref is -inf until then (-inf - -inf is no number, and not above)
-        const bool raise = mx - m_ref > RESCALE_THRESHOLD;
+        bool raise = mx - m_ref > RESCALE_THRESHOLD;
+        if (j == 0) {
+          // It starts at 0 and stays there if the row's first maximum lies in [0, 8], so that the largest P is 1 or more (one
+          // exponential pass less for a tile: chunks with a window of 64 94 -> 91 us); -inf until a row has seen a key.
+          raise |= mx < 0.f && mx > -CUDART_INF_F;
+          if (mx == -CUDART_INF_F) m_ref = mx;
+        }
         if (__any_sync(0xffffffffu, raise)) {
+          const bool scale_o = j > 0 && __any_sync(0xffffffffu, raise && m_ref > -CUDART_INF_F);      // else O is nothing yet
           const float alpha = raise ? fast_exp2(m_ref - mx) : 1.f;
           if (raise) m_ref = mx;
-          if (j > 0) {
+          if (scale_o) {
             // O may be rescaled only once P_{j-1} V_{j-1} has retired (its barrier completes again only with a later block's P V,
             // which waits for this one's P: the parity is exact).
             ok = mbar_wait(&pv_done[(j - 1) % STAGES], ((j - 1) / STAGES) & 1, abort_flag, p.status, 59, j);
@@ -547,7 +552,7 @@ packed_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
             }
             tmem_wait_st();
           }
-          l_sum *= alpha;
+          if (j > 0) l_sum *= alpha;
           sum = weigh(m_ref);
         }
         l_sum += sum;

@@ -208,6 +208,13 @@ def test_large_scores(cuda_device):
     b.check(b.run(cap=20.0), cap=20.0)                       # scores on both sides of the cap
 
 
+@pytest.mark.parametrize("size", [-12.0, -0.05, 12.0])
+def test_scores_of_one_sign(cuda_device, size):
+    b = Groups(cuda_device, [20], [700], list(range(20)), dtype=FP)
+    b.q, b.k = b.q.abs() * size, b.k.abs()
+    b.check(b.run())
+
+
 @pytest.mark.parametrize("cap", [None, 20.0, float("inf")])
 def test_no_numbers_in_visible_places(cuda_device, cap):
     """Heads of q that are no number, a key of a prefix and one of a sequence: their rows of the output are none either, and no

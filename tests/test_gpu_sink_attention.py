@@ -300,6 +300,15 @@ def test_large_scores_and_infinite_values_behind_the_window(cuda_device):
         b.check(b.run(cap=20.0), cap=20.0)                   # scores on both sides of the cap
 
 
+@pytest.mark.parametrize("new", [[1, 1], [70, 3]])
+@pytest.mark.parametrize("size", [-12.0, -1.0, -0.05, 0.0, 0.05, 1.0, 12.0])
+def test_scores_of_one_sign(cuda_device, new, size):
+    """All scores of a row far below zero (about -60, -5, -0.3) or above: the reference that P is taken against has to follow."""
+    b = Batch(cuda_device, new, [500, 300], 150, 5, dtype=FP, poison=False)
+    b.q, b.k = b.q.abs() * size, b.k.abs()
+    b.check(b.run())
+
+
 @pytest.mark.parametrize("new", [[1, 1, 1], [70, 3, 20]])
 @pytest.mark.parametrize("cap", [1e6, 1e30, float("inf")])
 def test_cap_far_above_the_scores(cuda_device, new, cap):
