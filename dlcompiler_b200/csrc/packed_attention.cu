@@ -19,7 +19,7 @@
 // softmax runs beside the other's matrix instructions.  192 threads: warp 4 issues the loads (K and V tiles of 64 keys, one
 // box per page, into rings of two, or of three where the rows fit half a tile: 24 sequences of 5 drafted tokens over 2048
 // keys 37 -> 32 us), one lane of warp 5 the tcgen05.mma (S_j = Q K_j^T into one of two S buffers, then O += P_{j-1} V_{j-1}
-// with P as the A operand from TMEM), warps 0-3 the softmax, one thread per row, with the exponentials taken against the
+// with P as the A operand from TMEM; three buffers and P_{j-2} with 64 columns), warps 0-3 the softmax, one thread per row, with the exponentials taken against the
 // old maximum before the block's own is known.  The blocks of 64 keys are those of the sinks and then those of the window;
 // blocks in between are skipped, and so are pages that hold no key which the tile sees.  Where the tiles are few, the CTAs
 // of a cluster share a tile's blocks and join through distributed shared memory.
@@ -44,13 +44,16 @@ constexpr int THREADS = 192;      // warps 0-3 softmax (TMEM quadrant = warp id)
 constexpr int WARP_TMA = 4;
 constexpr int WARP_MMA = 5;
 constexpr int KV_BOX = BN * 128;  // one 64-wide (128 B) column box of a K or V block
-constexpr int TMEM_COLS = 256;    // S0 [0,64) S1 [64,128), P over the first half of its S; O [128,128+D)
+constexpr int TMEM_COLS = 256;    // S buffers of 64 columns, P over the first half of its S, then O
 constexpr float RESCALE_THRESHOLD = 8.0f;   // log2 units: P stays below 2^8, well inside fp16
 enum { PREFILL, PREFIX };
-// ROWS of Q in shared memory, 128 or 64; the half that 64 leave free is a third pair of K and V buffers
+// ROWS of Q in shared memory, 128 or 64; the half that 64 leave free is a third pair of K and V buffers.  With 64 columns there is
+// room for four pairs, and beside O for a third S, so that Q K^T runs two blocks ahead of P V (256 sequences behind 32768 tokens:
+// 135 -> 126 us; prompts the same, whose softmax warps are never idle there).
 template <int D, int ROWS> struct Layout {
   static constexpr int BOXES = D / 64;
-  static constexpr int STAGES = ROWS == 64 ? 3 : 2;
+  static constexpr int S_BUFS = D == 64 ? 3 : 2;
+  static constexpr int STAGES = D == 64 ? 4 : ROWS == 64 ? 3 : 2;
   static constexpr int Q_BOX = ROWS * 128;                    // one 64-wide column box of the Q tile
   static constexpr int KV_BYTES = BOXES * KV_BOX;             // one K or V block
   static constexpr int OFF_Q = 0;
@@ -158,7 +161,7 @@ packed_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
                         const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ PackedParams p) {
   using namespace pa;
   using L = Layout<D, ROWS>;
-  constexpr int BOXES = L::BOXES, KV_BYTES = L::KV_BYTES, Q_BOX = L::Q_BOX, STAGES = L::STAGES;
+  constexpr int BOXES = L::BOXES, KV_BYTES = L::KV_BYTES, Q_BOX = L::Q_BOX, STAGES = L::STAGES, S_BUFS = L::S_BUFS;
   constexpr int OFF_Q = L::OFF_Q, OFF_K = L::OFF_K, OFF_V = L::OFF_V, OFF_CTRL = L::OFF_CTRL;
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -223,15 +226,15 @@ packed_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
       p.status[1] = 50;
     return;
   }
-  // block j uses the K and V buffers j % STAGES and waits for parity (j / STAGES) & 1 of their barriers; S and P have two buffers
+  // block j uses the K and V buffers j % STAGES and waits for parity (j / STAGES) & 1 of their barriers; S and P have S_BUFS buffers
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + OFF_CTRL);
   uint64_t* q_full = bars + 0;
   uint64_t* k_full = bars + 1;               // [STAGES]
   uint64_t* v_full = k_full + STAGES;        // [STAGES]
   uint64_t* qk_done = v_full + STAGES;       // [STAGES] S there; K buffer reusable
   uint64_t* pv_done = qk_done + STAGES;      // [STAGES] O updated; V buffer reusable
-  uint64_t* p_full = pv_done + STAGES;       // [2] P written
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(p_full + 2);
+  uint64_t* p_full = pv_done + STAGES;       // [S_BUFS] P written
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(p_full + S_BUFS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   if (warp == WARP_TMA && lane == 0) {
@@ -242,7 +245,7 @@ packed_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
       mbar_init(&qk_done[h], 1);
       mbar_init(&pv_done[h], 1);
     }
-    for (int h = 0; h < 2; ++h) mbar_init(&p_full[h], 128);
+    for (int h = 0; h < S_BUFS; ++h) mbar_init(&p_full[h], 128);
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -260,7 +263,7 @@ packed_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
     tc_fence_after_sync();
   }
   const uint32_t tmem_base = warp == WARP_TMA ? 0u : *tmem_slot;
-  const uint32_t tmem_o = tmem_base + 128;
+  const uint32_t tmem_o = tmem_base + S_BUFS * BN;
 
   float m_ref = 0.f, l_sum = 0.f;                  // softmax warps: reference maximum (scaled, base-2 domain) and sum
   const int row = threadIdx.x;                     // row of the tile == TMEM lane
@@ -336,7 +339,7 @@ packed_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
     }
   } else if (warp == WARP_MMA) {
     // ------------------------------ MMA issuer ------------------------------
-    // One thread's MMAs run in the order of their issue, so S_{j+2} overwrites P_j only once P_j V_j has read it.
+    // One thread's MMAs run in the order of their issue, so an S overwrites the P before it in its buffer only once P V has read that.
     if (lane == 0 && nb > 0) {
       bool ok = mbar_wait(q_full, 0, abort_flag, p.status, 53, 0);
       const uint64_t q_d0 = make_smem_desc(smem_u32(smem + OFF_Q), 16, 1024, 2);
@@ -345,7 +348,8 @@ packed_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
       const uint64_t v_d0 = make_smem_desc(smem_u32(smem + OFF_V), KV_BOX, 1024, 2);
       const uint32_t q_lo0 = (uint32_t)q_d0, k_lo0 = (uint32_t)k_d0, kq_hi = (uint32_t)(q_d0 >> 32);
       const uint32_t v_lo0 = (uint32_t)v_d0, v_hi = (uint32_t)(v_d0 >> 32);
-      for (int j = 0; ok && j <= nb; ++j) {
+      constexpr int AHEAD = S_BUFS - 1;                        // P V comes that many blocks after Q K^T
+      for (int j = 0; ok && j < nb + AHEAD; ++j) {
         if (j < nb) {
           // S_j = Q K_j^T
           const int s = j % STAGES;
@@ -356,18 +360,18 @@ packed_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
           for (int ks = 0; ks < D / 16; ++ks) {
             const uint32_t qoff = (uint32_t)(((ks >> 2) * Q_BOX + (ks & 3) * 32) >> 4);
             const uint32_t koff = (uint32_t)(((ks >> 2) * KV_BOX + (ks & 3) * 32) >> 4);
-            if (ks == 0) umma_ss_lohi<0>(tmem_base + (j & 1) * BN, q_lo0 + qoff, kq_hi, k_lo + koff, kq_hi, p.idesc_qk);
-            else umma_ss_lohi<1>(tmem_base + (j & 1) * BN, q_lo0 + qoff, kq_hi, k_lo + koff, kq_hi, p.idesc_qk);
+            if (ks == 0) umma_ss_lohi<0>(tmem_base + (j % S_BUFS) * BN, q_lo0 + qoff, kq_hi, k_lo + koff, kq_hi, p.idesc_qk);
+            else umma_ss_lohi<1>(tmem_base + (j % S_BUFS) * BN, q_lo0 + qoff, kq_hi, k_lo + koff, kq_hi, p.idesc_qk);
           }
           umma_commit(&qk_done[s]);
         }
-        if (j > 0) {
-          // O += P_{j-1} V_{j-1}
-          const int jj = j - 1, s = jj % STAGES;
-          const uint32_t p_ph = (jj >> 1) & 1, v_ph = (jj / STAGES) & 1, pt = tmem_base + (jj & 1) * BN;
-          const bool r1 = mbar_try_wait(&p_full[jj & 1], p_ph), r2 = mbar_try_wait(&v_full[s], v_ph);
+        if (j >= AHEAD) {
+          // O += P V of block jj
+          const int jj = j - AHEAD, s = jj % STAGES, u = jj % S_BUFS;
+          const uint32_t p_ph = (jj / S_BUFS) & 1, v_ph = (jj / STAGES) & 1, pt = tmem_base + u * BN;
+          const bool r1 = mbar_try_wait(&p_full[u], p_ph), r2 = mbar_try_wait(&v_full[s], v_ph);
           if (!(r1 && r2)) {
-            if (!mbar_wait(&p_full[jj & 1], p_ph, abort_flag, p.status, 56, jj)) break;
+            if (!mbar_wait(&p_full[u], p_ph, abort_flag, p.status, 56, jj)) break;
             if (!mbar_wait(&v_full[s], v_ph, abort_flag, p.status, 57, jj)) break;
           }
           tc_fence_after_sync();
@@ -400,7 +404,7 @@ packed_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after_sync();
-      const uint32_t s_cols = tmem_base + lane_field + (j & 1) * BN;
+      const uint32_t s_cols = tmem_base + lane_field + (j % S_BUFS) * BN;
       const int key0 = block_key(j);
       // does every row of the warp see the whole block?
       const bool whole = MODE == PREFILL ? key0 + BN <= whole_to && (key0 >= whole_from || key0 + BN <= p.sinks) : key0 + BN <= keys;
@@ -578,7 +582,7 @@ packed_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
       }
       tmem_wait_st();
       tc_fence_before_sync();
-      mbar_arrive(&p_full[j & 1]);
+      mbar_arrive(&p_full[j % S_BUFS]);
     }
     if (ok && nb > 0) {
       ok = mbar_wait(&pv_done[(nb - 1) % STAGES], ((nb - 1) / STAGES) & 1, abort_flag, p.status, 60, nb);
