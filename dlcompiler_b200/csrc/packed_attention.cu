@@ -19,10 +19,10 @@
 // softmax runs beside the other's matrix instructions.  192 threads: warp 4 issues the loads (K and V tiles of 64 keys, one
 // box per page, into rings of two, or of three where the rows fit half a tile: 24 sequences of 5 drafted tokens over 2048
 // keys 37 -> 32 us), one lane of warp 5 the tcgen05.mma (S_j = Q K_j^T into one of two S buffers, then O += P_{j-1} V_{j-1}
-// with P as the A operand from TMEM; three buffers and P_{j-2} with 64 columns), warps 0-3 the softmax, one thread per row, with the exponentials taken against the
-// old maximum before the block's own is known.  The blocks of 64 keys are those of the sinks and then those of the window;
-// blocks in between are skipped, and so are pages that hold no key which the tile sees.  Where the tiles are few, the CTAs
-// of a cluster share a tile's blocks and join through distributed shared memory.
+// with P as the A operand from TMEM; three buffers and P_{j-2} with 64 columns), warps 0-3 the softmax, one thread per row,
+// with the exponentials taken against the old maximum before the block's own is known.  The blocks of 64 keys are those of
+// the sinks and then those of the window; blocks in between are skipped, and so are pages that hold no key which the tile
+// sees.  Where the tiles are few, the CTAs of a cluster share a tile's blocks and join through distributed shared memory.
 //
 // Bound by the chain S_j -> P_j -> P V -> S_{j+2}: a softmax warp takes about 1220 clocks for a block, the way from a P
 // written to the S after next 1890, with the tensor pipe 54 %, the exponential unit 56 % and the issue slots 46 % busy (one

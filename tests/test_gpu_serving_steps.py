@@ -134,3 +134,49 @@ def test_answers_behind_one_prompt_in_a_graph(cuda_device):
             close(got[b:b + 1], ref, bound, f"step {t}, sequence {b}")
             close(other[b:b + 1], ref, bound, f"whole context, step {t}, sequence {b}")
     check_device_status()
+
+
+@pytest.mark.parametrize("streams", [1, 3])
+def test_calls_from_several_threads(cuda_device, streams):
+    """Threads that call at the same time, on streams of their own or with their launches mixed on one: the bits of one after
+    the other."""
+    import threading
+
+    dtype, batch = torch.bfloat16, 6
+    servers, refs = [], []
+    for seed in range(3):
+        s = Server(cuda_device, batch, 60, 8, dtype, 10 + seed)
+        s.k.copy_(torch.randn(s.k.shape, generator=s.g)), s.v.copy_(torch.randn(s.v.shape, generator=s.g))
+        for b in range(batch):
+            s.need(s.table, b, 8 * PAGE)
+        s.q = torch.randn(batch, HQ, D, generator=s.g).to(dtype).to(s.dev)
+        s.lens, s.start, s.one = _ints([5 + 20 * b for b in range(batch)], s.dev), _ints(range(batch), s.dev), _ints([1] * batch, s.dev)
+        servers.append(s)
+
+    def step(s):
+        q, _ = s.rotated(s.q, s.q[:, :2], s.lens.long().repeat(3, 1))
+        a = sink_attention_fwd(q, s.k, s.v, torch.empty_like(q), s.table, s.start, s.one, s.lens, 1, 31, 4)
+        b = sink_attention_fwd(q, s.k, s.v, torch.empty_like(q), s.table, s.start, s.one, s.lens, 2, 31, 4)
+        c = shared_prefix_attention_fwd(q, s.k, s.v, torch.empty_like(q), s.table[:2], s.lens[4:], _ints([0, 2, 6], s.dev),
+                                        s.table, s.lens)
+        return a, b, c
+
+    refs = [step(s) for s in servers]
+    torch.cuda.synchronize()
+    pool = [torch.cuda.Stream() for _ in range(streams)]
+    wrong = []
+
+    def work(i):
+        with torch.cuda.stream(pool[i % streams]):
+            for _ in range(50):
+                got = step(servers[i])
+                if not all(torch.equal(x, y) for x, y in zip(got, refs[i])):
+                    wrong.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+    check_device_status()
