@@ -395,8 +395,9 @@ packed_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
     // A warp whose rows are all past the tile's last one keeps in step and computes nothing: its P and O stay what they are, and
     // no other row reads them.
     const bool busy = warp * 32 < tile_rows;
-    // what every row of the warp sees, but for the sinks
-    const int whole_to = min(keys, hist + q0 + (int)((uint32_t)(warp * 32) * p.group_inv >> 16) + 1);
+    // what every row of the warp sees, but for the sinks; never past what the tile sees, so that a warp without rows also zeroes
+    // its V rows there
+    const int whole_to = min(vis_hi, hist + q0 + (int)((uint32_t)(warp * 32) * p.group_inv >> 16) + 1);
     const int whole_from = hist + q0 + (int)((uint32_t)(max(min(warp * 32 + 32, tile_rows), 1) - 1) * p.group_inv >> 16) - p.window;
     for (int j = 0; j < nb; ++j) {
       const int s = j % STAGES;

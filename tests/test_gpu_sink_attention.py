@@ -355,3 +355,27 @@ def test_empty_calls(cuda_device):
     b.o.fill_(7)
     b.run(most=0)
     assert (b.o == 7).all() and dl.is_built()
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+@pytest.mark.parametrize("hq,past", [(43, 1), (48, 1), (65, 0), (71, 0), (96, 5)])
+def test_no_number_behind_a_tile(cuda_device, hq, past, value):
+    """43 to 48 or 65 to 96 q-heads to a kv head leave the last warp of a tile without rows.  The token after a tile, at the end of
+    a block of 64 keys, is fetched with it and seen by nobody there: its values change no bit of the rows in front."""
+    b = Batch(cuda_device, [70], [past], 1000, 4, hq=hq, hkv=1, poison=False)
+    ref = b.run().clone()
+    b.v.view(-1, 1, 64)[rows_of(b.clean[0], 64, 16)[63]] = value
+    o = b.run(o=torch.empty_like(b.o))
+    assert torch.equal(o[:63 - past], ref[:63 - past]) and not o[63 - past:].isfinite().any()
+
+
+@pytest.mark.parametrize("page", [16, 64])
+def test_sequences_past_max_seqlen(cuda_device, page):
+    """Tiles as for two tokens, half of whose warps have no rows, and a sequence of 200; what lies in shared memory from the call
+    before, here no numbers, is nobody's value."""
+    b = Batch(cuda_device, [200, 7, 90], [40, 0, 13], 1000, 4, page=page, hq=4, hkv=4)
+    v = b.v
+    b.v = torch.full_like(v, float("nan"))
+    assert b.run(most=2).isnan().all()
+    b.v = v
+    b.check(b.run(most=2))
