@@ -88,19 +88,20 @@ cluster_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
   // ---- the sequence: its row of q, its keys ----
   const int page_size = 1 << p.page_shift;
   int64_t row = b;
-  int ctx = clamped_index(p.kv_lens, b, p.lens_is_int64);
+  int64_t len = clamped_index(p.kv_lens, b, p.lens_is_int64);
   if (!PREFIX) {
     const int q_len = clamped_index(p.q_lens, b, p.qlens_is_int64);
     row = clamped_index(p.q_start, b, p.start_is_int64);
     if (q_len <= 0 || row < 0 || row >= p.tokens) return;    // the whole cluster leaves
-    ctx -= q_len - 1;                                        // its first token (there is one)
+    len -= q_len - 1;                                        // its first token (there is one)
   }
-  ctx = (int)min((int64_t)ctx, (int64_t)p.max_pages << p.page_shift);
-  const int lo = (p.window >= 0 && ctx - 1 > p.window) ? ctx - 1 - p.window : 0;
+  // the keys that are there; a query past them keeps its position
+  const int ctx = (int)max((int64_t)0, min(len, (int64_t)p.max_pages << p.page_shift));
+  const int lo = p.window >= 0 ? (int)max((int64_t)0, min(len - 1 - p.window, (int64_t)ctx)) : 0;
   const int sink_end = min(p.sinks, lo);
   const int base = lo & ~(TILE - 1);
   const int sink_tiles = (sink_end + TILE - 1) / TILE;
-  const int tiles = ctx > 0 ? sink_tiles + (ctx - base + TILE - 1) / TILE : 0;
+  const int tiles = sink_tiles + (ctx > lo ? (ctx - base + TILE - 1) / TILE : 0);
   const int t_lo = (int)((int64_t)tiles * rank / cluster), t_hi = (int)((int64_t)tiles * (rank + 1) / cluster);
   // tile t starts at key `at` and the keys [from, to) count
   auto tile_keys = [&](int t, int& at, int& from, int& to) {

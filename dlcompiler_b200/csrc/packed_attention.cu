@@ -199,8 +199,7 @@ packed_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
     vis_hi = max(0, min(keys, pos_hi + 1));
     first_block = vis_lo / BN;
     sink_blocks = min((min(p.sinks, vis_hi) + BN - 1) / BN, first_block);
-    nb = max(0, (vis_hi + BN - 1) / BN - first_block);
-    nb = nb > 0 ? nb + sink_blocks : 0;
+    nb = sink_blocks + max(0, (vis_hi + BN - 1) / BN - first_block);
   } else {
     if (split * p.prefix.chunk >= keys) return;
     first_block = split * (p.prefix.chunk / BN);

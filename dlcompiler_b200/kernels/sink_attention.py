@@ -76,7 +76,8 @@ def sink_attention_fwd(
     int32 or int64.  `max_seqlen` is the largest of `q_seqlens`: 1 takes the form for single tokens (sequences with
     none are left out, of longer ones only the first token is computed), anything larger the one for chunks of prompts or
     several drafted tokens, any mixture of lengths.  Rows of `q` and `o` that belong to no sequence are left as they are; a
-    query that sees no key gets zeros.
+    query that sees no key gets zeros.  Where `kv_seqlens` is past what a row of `block_offsets` has room for, queries keep their
+    positions and the tokens past the table are not there.
 
     Only pages with a token that some query of a tile of 128 rows sees are looked at: entries of `block_offsets` for
     tokens behind the window may be stale.  A page outside the cache where a visible token should be is an error

@@ -294,7 +294,8 @@ int dlb_paged_decode_rows(const void* q, const void* k_cache, const void* v_cach
  * [total_q_tokens, hq, head_dim_v], caches [num_pages, page_size, hkv, d] (page_size a power of two >= 16) that already
  * hold the new tokens, block_table [batch, max_pages], kv_seq_len [batch] with the new tokens; every index array int32
  * or int64.  max_q_len is the largest of q_seq_len; 1 selects the form for single tokens.  Rows of no sequence are not
- * written, queries without a key get zeros, pages without a visible token are not looked at.  softcap > 0: scores become
+ * written, queries without a key get zeros, pages without a visible token are not looked at; where kv_seq_len is past the
+ * table's room, positions stay and the tokens past the table are not there.  softcap > 0: scores become
  * softcap * tanh(score * sm_scale / softcap), softcap >= 1e-8 sm_scale.  hq / hkv <= 128, head sizes multiples of 8 up
  * to 128, fp16 / bf16, sm_scale > 0, rows of q, out and the caches 16-byte aligned.  The reference has the window without sinks
  * (python/dlBLAS/dlblas/kernels/paged_attention.py:421-424, 447). */

@@ -379,3 +379,25 @@ def test_sequences_past_max_seqlen(cuda_device, page):
     assert b.run(most=2).isnan().all()
     b.v = v
     b.check(b.run(most=2))
+
+
+@pytest.mark.parametrize("most", [1, 3])
+@pytest.mark.parametrize("window,sinks", [(40, 5), (40, 0), (33, 70), (0, 100)])
+def test_lengths_past_the_table(cuda_device, most, window, sinks):
+    """A query keeps its position, and the tokens that the table has no room for are not there, in both forms."""
+    b = Batch(cuda_device, [most] * 5, [60, 93, 130, 200, 400], window, sinks, poison=False)
+    b.table = b.clean[:, :6].int()
+    o, k, v = b.run(), b.k.view(-1, 2, 64), b.v.view(-1, 2, 64)
+    for s in range(5):
+        n = min(b.past[s] + most, 96)
+        rows = rows_of(b.clean[s], n, 16)
+        ref, bound = attend(b.q[s * most:(s + 1) * most], k[rows], v[rows], b.seen(s, cuda_device)[:, :n], 64 ** -0.5, 0.0, BF)
+        close(o[s * most:(s + 1) * most], ref, bound, f"sequence {s}")
+
+
+def test_first_token_of_a_sequence_before_the_cache(cuda_device):
+    """max_seqlen 1 and sequences of two tokens: a length far below zero has no key."""
+    b = Batch(cuda_device, [2, 2], [40, 50], 30, 4, idx=torch.int64, poison=False)
+    b.kv[1] = -2 ** 40
+    o = b.run(most=1)
+    assert not o[2].any() and (o[[1, 3]] == 7).all() and o[0].any()
