@@ -195,7 +195,7 @@ packed_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
   int vis_lo = 0, vis_hi = keys, pos_hi = 0, sink_blocks = 0, first_block, nb;
   if (MODE == PREFILL) {
     pos_hi = hist + min(q0 + p.tile_tokens, n) - 1;
-    vis_lo = max(0, hist + q0 - p.window);
+    vis_lo = max(0, max(0, hist + q0) - p.window);           // (a window may be as long as an int)
     vis_hi = max(0, min(keys, pos_hi + 1));
     first_block = vis_lo / BN;
     sink_blocks = min((min(p.sinks, vis_hi) + BN - 1) / BN, first_block);
@@ -387,6 +387,8 @@ packed_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
     // ------------------------------ softmax / correction ------------------------------
     const bool live = row < tile_rows;
     const int q_pos = hist + q0 + (int)((uint32_t)row * p.group_inv >> 16);      // position of this row's token
+    auto first_key = [&](int pos) { return max(0, max(0, pos) - p.window); };    // of its window
+    const int q_from = first_key(q_pos);
     const float cap_in = CAP ? 2.f * 1.4426950408889634f * p.sm_scale / p.softcap : 0.f, cap_out = p.softcap * 1.4426950408889634f,
                 cap_x = CAP ? p.sm_scale / p.softcap : 0.f;
     const float eff_scale = CAP ? 1.f : p.scale_log2;
@@ -397,7 +399,7 @@ packed_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
     // what every row of the warp sees, but for the sinks; never past what the tile sees, so that a warp without rows also zeroes
     // its V rows there
     const int whole_to = min(vis_hi, hist + q0 + (int)((uint32_t)(warp * 32) * p.group_inv >> 16) + 1);
-    const int whole_from = hist + q0 + (int)((uint32_t)(max(min(warp * 32 + 32, tile_rows), 1) - 1) * p.group_inv >> 16) - p.window;
+    const int whole_from = first_key(hist + q0 + (int)((uint32_t)(max(min(warp * 32 + 32, tile_rows), 1) - 1) * p.group_inv >> 16));
     for (int j = 0; j < nb; ++j) {
       const int s = j % STAGES;
       ok = mbar_wait(&qk_done[s], (j / STAGES) & 1, abort_flag, p.status, 58, j);
@@ -433,7 +435,7 @@ packed_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
           const int hi = MODE == PREFILL ? min(q_pos, keys - 1) - key0 : keys - 1 - key0;      // last visible key
           uint64_t bits = hi < 0 ? 0ull : hi >= BN - 1 ? ~0ull : (2ull << hi) - 1;
           if (MODE == PREFILL) {
-            const int lo = q_pos - p.window - key0, sk = p.sinks - key0;
+            const int lo = q_from - key0, sk = p.sinks - key0;
             const uint64_t win = lo <= 0 ? ~0ull : lo >= BN ? 0ull : ~0ull << lo;
             const uint64_t snk = sk <= 0 ? 0ull : sk >= BN ? ~0ull : (1ull << sk) - 1;
             bits &= win | snk;
@@ -816,7 +818,8 @@ extern "C" int dlb_sink_attention(const void* q, const void* k_cache, const void
                 "sink_attention: null pointer");
   rc = check_rows("sink_attention", q, out, q_stride_t, q_stride_h, o_stride_t, o_stride_h);
   if (rc != DLB_OK) return rc;
-  const int win = (int)(window < (1 << 30) ? window : (1 << 30)), snk = (int)(sinks < (1 << 30) ? sinks : (1 << 30));
+  const int win = (int)(window < INT_MAX ? window : INT_MAX), snk = (int)(sinks < INT_MAX ? sinks : INT_MAX);
+  const int64_t most_keys = (int64_t)win + snk, room = max_pages * page_size;
   cudaStream_t s = (cudaStream_t)stream;
   if (max_q_len == 1) {
     ClusterDecodeParams d = {};
@@ -827,7 +830,7 @@ extern "C" int dlb_sink_attention(const void* q, const void* k_cache, const void
     d.page_shift = log2_of(page_size); d.max_pages = (int)max_pages; d.num_pages = (int)num_pages;
     d.table_is_int64 = table_is_int64; d.lens_is_int64 = kvlen_is_int64; d.start_is_int64 = start_is_int64; d.qlens_is_int64 = qlen_is_int64;
     d.window = win; d.sinks = snk; d.sm_scale = sm_scale; d.softcap = softcap; d.status = status;
-    const int64_t bound = window + sinks + 1 < max_pages * page_size ? window + sinks + 1 : max_pages * page_size;
+    const int64_t bound = most_keys + 1 < room ? most_keys + 1 : room;
     return launch_cluster_decode(d, k_cache, v_cache, k_stride_page, k_stride_slot, k_stride_head, v_stride_page,
                                  v_stride_slot, v_stride_head, width, bound, dtype, s);
   }
@@ -843,7 +846,7 @@ extern "C" int dlb_sink_attention(const void* q, const void* k_cache, const void
   const int64_t tiles = total_q_tokens / p.tile_tokens + batch;      // sequences end inside a tile at most once each
   DLB_CHECK_ARG(tiles * hkv * MAX_CLUSTER < (1LL << 31), DLB_ERR_TOO_LARGE, "sink_attention: grid too large");
   p.tiles = (int)tiles;
-  const int64_t seen = window + p.tile_tokens + sinks < max_pages * page_size ? window + p.tile_tokens + sinks : max_pages * page_size;
+  const int64_t seen = most_keys + p.tile_tokens < room ? most_keys + p.tile_tokens : room;
   const int64_t likely = batch * ((total_q_tokens / batch + p.tile_tokens - 1) / p.tile_tokens);      // with sequences of one length
   p.cluster = pick_packed_cluster((likely < tiles ? likely : tiles) * hkv, (seen + pa::BN - 1) / pa::BN);
   CUtensorMap tq, tk, tv;

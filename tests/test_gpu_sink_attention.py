@@ -401,3 +401,20 @@ def test_first_token_of_a_sequence_before_the_cache(cuda_device):
     b.kv[1] = -2 ** 40
     o = b.run(most=1)
     assert not o[2].any() and (o[[1, 3]] == 7).all() and o[0].any()
+
+
+@pytest.mark.parametrize("most", [1, 3])
+def test_window_past_2_30(cuda_device, most):
+    """Positions past 2^30 over a table of 112 tokens: the window is not cut short."""
+    b = Batch(cuda_device, [most] * 2, [100, 90], 0, 3, poison=False)
+    for window in (2 ** 30 + 180, 2 ** 31 - 1):
+        b.window = window
+        b.kv = torch.tensor([min(window + n, 2 ** 31 - 1) for n in (20, 60)], dtype=torch.int32, device=cuda_device)
+        b.table = b.clean.int()[:, :6]
+        o = b.run(o=torch.empty_like(b.o))
+        k, v = b.k.view(-1, 2, 64), b.v.view(-1, 2, 64)
+        for s, kv in enumerate(b.kv.tolist()):
+            pos, key = torch.arange(kv - most, kv, device=cuda_device)[:, None], torch.arange(96, device=cuda_device)
+            rows = rows_of(b.clean[s], 96, 16)
+            ref, bound = attend(b.q[s * most:(s + 1) * most], k[rows], v[rows], (key >= pos - window) | (key < 3), 64 ** -0.5, 0.0, BF)
+            close(o[s * most:(s + 1) * most], ref, bound, f"window {window}, sequence {s}")
