@@ -720,6 +720,11 @@ static int launch_packed(const CUtensorMap& tq, const CUtensorMap& tk, const CUt
                   : launch_packed_x<__half, 64, MODE>(tq, tk, tv, p, grid, s);
 }
 
+// Keys are counted in 32 bits, by the loading warps up to 64 blocks of 64 past the last one.
+static bool too_long(int64_t max_pages, int64_t page_size) {
+  return max_pages >= (1LL << 31) || max_pages * page_size > INT_MAX - 8192;
+}
+
 // What both entry points take: types, head sizes, cache layout.  Returns DLB_OK or an error; `width` is the tile width.
 static int check_attention(const char* what, int64_t batch, int64_t tokens, int64_t hq, int64_t hkv, int64_t head_dim,
                            int64_t head_dim_v, int64_t page_size, int64_t num_pages, int64_t max_pages, float sm_scale,
@@ -736,7 +741,7 @@ static int check_attention(const char* what, int64_t batch, int64_t tokens, int6
   DLB_CHECK_ARG(page_size >= 16 && page_size <= (1 << 30) && (page_size & (page_size - 1)) == 0, DLB_ERR_UNSUPPORTED,
                 "%s: page size %lld must be a power of two from 16 on", what, (long long)page_size);
   DLB_CHECK_ARG(num_pages >= 1 && max_pages >= 1, DLB_ERR_BAD_ARG, "%s: empty cache or table", what);
-  DLB_CHECK_ARG(num_pages < (1LL << 31) && max_pages * page_size < (1LL << 31) && tokens * hq < (1LL << 31) &&
+  DLB_CHECK_ARG(num_pages < (1LL << 31) && !too_long(max_pages, page_size) && tokens * hq < (1LL << 31) &&
                     batch <= 65535 && hkv * ((hq / hkv + 15) / 16) <= 65535,
                 DLB_ERR_TOO_LARGE, "%s: sizes past 31 bits", what);
   if (softcap > FLT_MAX) softcap = 0.f;       // as good as none
@@ -882,8 +887,7 @@ extern "C" int dlb_shared_prefix_attention(
   int rc = check_attention("shared_prefix_attention", batch, batch, hq, hkv, head_dim, head_dim_v, page_size, num_pages,
                            max_pages < prefix_max_pages ? max_pages : prefix_max_pages, sm_scale, softcap, dtype, width);
   if (rc != DLB_OK) return rc;
-  DLB_CHECK_ARG(groups >= 1 && groups <= 65535 && prefix_max_pages * page_size < (1LL << 31) &&
-                    max_pages * page_size < (1LL << 31),
+  DLB_CHECK_ARG(groups >= 1 && groups <= 65535 && !too_long(prefix_max_pages, page_size) && !too_long(max_pages, page_size),
                 DLB_ERR_TOO_LARGE, "shared_prefix_attention: number of groups or length of a table out of range");
   DLB_CHECK_ARG(chunk >= 64 && chunk % 64 == 0 && chunk < (1LL << 31), DLB_ERR_BAD_ARG,
                 "shared_prefix_attention: chunk %lld must be a multiple of 64", (long long)chunk);

@@ -160,3 +160,15 @@ def test_prefix_split_rule():
     assert _pick_prefix_split(5000, 1, 8, 512) == (512 * 64, 1)
     chunk, cluster = _pick_prefix_split(8, 1, 8, 1876)
     assert 148 < 8 * cluster * -(-1876 * 64 // chunk) <= 224
+
+
+def test_tables_that_end_near_2_31_tokens():
+    """Keys are counted in 32 bits, some blocks past a table's end."""
+    lib = _lib.load()
+    for columns in ((1 << 27) - 1, (1 << 27) - 512, 1 << 62):
+        assert lib.dlb_sink_attention(16, 16, 16, 16, 16, 16, 16, 16, 3, 3, 1, 4, 2, 64, 64, 16, 4, columns, 256, 64, 256, 64, 2048,
+                                      128, 64, 2048, 128, 64, 2, 0, 0, 0, 0, 8, 2, 0.1, -1.0, _lib.DTYPE_BF16, None, None) == -5
+        for prefix, own in ((2, columns), (columns, 2)):
+            assert lib.dlb_shared_prefix_attention(16, 16, 16, 16, 16, 16, 16, 16, 16, 16, 3, 2, 4, 2, 64, 64, 16, 4, prefix, own, 256,
+                                                   64, 256, 64, 2048, 128, 64, 2048, 128, 64, 2, 2, 0, 0, 0, 0, 0, 64, 1, 0.1, -1.0,
+                                                   _lib.DTYPE_BF16, None, None) == -5
