@@ -65,7 +65,7 @@ __device__ __forceinline__ void report_bad_page(int* status, int row, int column
 
 // Splits of a prefix of `len` tokens (as many as the table has room for).
 __device__ __forceinline__ int prefix_splits(const PrefixPartials& p, int len) {
-  return (max(min(len, p.max_len), 0) + p.chunk - 1) / p.chunk;
+  return (int)(((uint32_t)max(min(len, p.max_len), 0) + (uint32_t)p.chunk - 1) / (uint32_t)p.chunk);    // the sum may pass 2^31
 }
 
 // Rows [start, start + n) of group g, kept inside the rows that exist.
