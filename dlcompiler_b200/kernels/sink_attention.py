@@ -73,7 +73,8 @@ def sink_attention_fwd(
     Arguments as in `paged_attention_fwd`: `q` [total_q, Hq, D] packed by `q_start_loc` / `q_seqlens`, caches `k` / `v`
     [num_pages, page_size, Hkv, D], which already hold the new tokens, `o` [total_q, Hq, Dv] written in place,
     `block_offsets` [batch, max_pages], `kv_seqlens` [batch] tokens in the cache, the new ones included; index tensors
-    int32 or int64.  `max_seqlen` is the largest of `q_seqlens`: 1 takes the form for single tokens (sequences with
+    int32 or int64.  Other than there, `window_size` has no value for no window (None and -1 are refused, one as long as the
+    longest context hides nothing), and 0 leaves the query's own token and the sinks.  `max_seqlen` is the largest of `q_seqlens`: 1 takes the form for single tokens (sequences with
     none are left out, of longer ones only the first token is computed), anything larger the one for chunks of prompts or
     several drafted tokens, any mixture of lengths.  Rows of `q` and `o` that belong to no sequence are left as they are; a
     query that sees no key gets zeros.  Where `kv_seqlens` is past what a row of `block_offsets` has room for, queries keep their
@@ -91,7 +92,8 @@ def sink_attention_fwd(
     batch = q_seqlens.numel()
     block_offsets, columns, bt_stride = rows_of_table(block_offsets, batch, "block_offsets")
     assert q_start_loc.numel() >= batch and kv_seqlens.numel() >= batch, "q_start_loc and kv_seqlens: one per sequence"
-    assert window_size >= 0 and num_sinks >= 0 and max_seqlen >= 0, "window_size, num_sinks and max_seqlen must not be negative"
+    assert window_size is not None and window_size >= 0 and num_sinks >= 0 and max_seqlen >= 0, \
+        "window_size, num_sinks and max_seqlen must not be negative (there is no window_size for none: pass the longest context)"
     q_start_loc, q_seqlens, kv_seqlens = q_start_loc.contiguous(), q_seqlens.contiguous(), kv_seqlens.contiguous()
     wide = (is64(block_offsets, "block_offsets"), is64(q_start_loc, "q_start_loc"), is64(q_seqlens, "q_seqlens"),
             is64(kv_seqlens, "kv_seqlens"))

@@ -172,3 +172,12 @@ def test_tables_that_end_near_2_31_tokens():
             assert lib.dlb_shared_prefix_attention(16, 16, 16, 16, 16, 16, 16, 16, 16, 16, 3, 2, 4, 2, 64, 64, 16, 4, prefix, own, 256,
                                                    64, 256, 64, 2048, 128, 64, 2048, 128, 64, 2, 2, 0, 0, 0, 0, 0, 64, 1, 0.1, -1.0,
                                                    _lib.DTYPE_BF16, None, None) == -5
+
+
+@pytest.mark.parametrize("window", [None, -1])
+def test_sink_attention_has_no_code_for_no_window(no_launch, window):
+    """paged_attention_fwd takes None and -1 for no window."""
+    args = _attention_args()
+    args.update(q_start_loc=torch.arange(3), q_seqlens=torch.ones(3, dtype=torch.int32), max_seqlen=1, num_sinks=2)
+    with pytest.raises(AssertionError, match="window_size"):
+        dl.sink_attention_fwd(**args, window_size=window)
