@@ -8,7 +8,7 @@
 //
 // HBM-bound: q and k are read and written once, and positions are a few bytes per token, where tables of cos and
 // sin would add 2 * dim elements per token.  The angles are formed in the kernel, once per token and frequency, and
-// shared by its heads: the product is taken in 64 bits, in turns, and only its fraction is kept, since at position
+// shared by its heads: the product is taken in turns, in twice 64 bits, and only its fraction is kept, since at position
 // 10^6 a 32-bit product is off by 0.06 rad; the sine and cosine of the fraction are 32-bit, with the rounding of
 // their argument put back to first order.  The rotation is 32-bit with one rounding at the store.
 #include "common.cuh"
@@ -38,6 +38,18 @@ template <typename T, int VEC> struct alignas(sizeof(T) * VEC) ElemVec {
   T v[VEC];
 };
 
+// What is left of pos * freq / (2 pi) turns without the whole ones, in [-1/2, 1/2].  Both products are carried in two parts, the
+// second the exact remainder of the first, and so is 1 / (2 pi): with single products the angle at position 2^31 is off by
+// 4e-7, seven roundings of a 32-bit result.  Off by 2^-54 of a turn up to position 2^40 and by 2^-43 up to 2^53, past which
+// whole numbers are no longer exact in 64 bits.
+__device__ __forceinline__ double fraction_of_turns(double pos, double freq) {
+  constexpr double TURN = 0x1.45f306dc9c883p-3, TURN_REST = -0x1.6b01ec5417056p-57;      // 1 / (2 pi), 0.159..., to 106 bits
+  const double angle = __dmul_rn(pos, freq), angle_rest = fma(pos, freq, -angle);
+  const double turns = __dmul_rn(angle, TURN), turns_rest = fma(angle, TURN, -turns);
+  const double part = (turns - rint(turns)) + (turns_rest + fma(angle, TURN_REST, angle_rest * TURN));
+  return part - rint(part);
+}
+
 // A CTA forms the cos / sin of TOK tokens in shared memory, then its threads walk the tokens' items: VEC columns of a head's
 // lower half and the matching ones of the upper half, or two vectors of the columns behind them.
 template <typename T, int VEC, int TOK>
@@ -58,8 +70,7 @@ __global__ void __launch_bounds__(mar::THREADS, VEC == 8 ? 6 : 8) multi_axis_rot
     const int64_t at = (int64_t)p.axis[f] * p.pos_stride + t0 + tl;
     const double pos = p.pos_is_int64 ? (double)reinterpret_cast<const int64_t*>(p.positions)[at]
                                       : (double)reinterpret_cast<const int32_t*>(p.positions)[at];
-    const double turns = pos * ((double)p.inv_freq[f] * 0.15915494309189533577);    // 1 / (2 pi)
-    const double part = 2.0 * (turns - rint(turns));                               // in half turns, [-1, 1]
+    const double part = 2.0 * fraction_of_turns(pos, (double)p.inv_freq[f]);        // in half turns
     const float x = (float)part;
     const float off = (float)(part - (double)x) * 3.14159265358979f;
     float s, c;

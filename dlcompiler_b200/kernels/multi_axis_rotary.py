@@ -103,8 +103,9 @@ def apply_multi_axis_rotary(
     up to dim / 2 and 256 of them) the angle per step of each frequency; the first `2 * len(inv_freq)` columns are
     rotated (column f with column f + len(inv_freq)), the others pass through.  `sections[a]` frequencies follow axis
     a: the first sections[0] frequencies the first axis and so on, or, with `interleaved`, one frequency to each axis
-    in turn, an axis dropping out once it has its number.  Angles are formed in 64 bits and the rotation in 32, with
-    one rounding to the tensors' type (fp16, bf16, fp32): no cos / sin tables, and positions far out stay exact.
+    in turn, an axis dropping out once it has its number.  Angles are formed in twice 64 bits and the rotation in 32, with
+    one rounding to the tensors' type (fp16, bf16, fp32): no cos / sin tables, and angles as good far out, up to position
+    2^53, as near 0.
 
     Differentiable in q and k where one of them requires a gradient; `q_embed` / `k_embed` (which may be the inputs)
     are for calls without one.  Returns (q_embed, k_embed).

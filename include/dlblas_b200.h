@@ -351,7 +351,7 @@ int dlb_apply_rotary(const void* q, const void* k, const void* cos, const void* 
  * (f, f + rot_dim / 2) of every head by positions[axis_of_freq[f]][token] * inv_freq[f], columns from rot_dim on pass
  * through; inverse != 0 turns back (the gradient).  positions int32 or int64 [axes, tokens] with position_stride
  * between axes (1 to 8 of them), inv_freq fp32 [rot_dim / 2], axis_of_freq a HOST array of rot_dim / 2 bytes that is
- * read during the call.  Angles in 64 bits, the rotation in 32, one rounding.  Outputs may be the inputs (same pointer
+ * read during the call.  Angles in twice 64 bits (positions up to 2^53), the rotation in 32, one rounding.  Outputs may be the inputs (same pointer
  * and strides); hq or hk may be 0.  No counterpart in the reference. */
 int dlb_multi_axis_rotary(const void* q, const void* k, void* q_out, void* k_out, const void* positions,
                           int positions_are_int64, int64_t position_stride, const float* inv_freq,

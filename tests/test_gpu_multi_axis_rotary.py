@@ -1,4 +1,7 @@
 """GPU: rotary positions of several axes against complex numbers in 64 bits, forward, gradient and refusals of layouts."""
+import math
+from fractions import Fraction
+
 import pytest
 import torch
 
@@ -186,3 +189,21 @@ def test_other_stream_and_graph(cuda_device):
     qe.zero_()
     graph.replay()
     assert torch.equal(qe, apply_multi_axis_rotary(q, k, pos, inv, [16, 8, 8])[0])
+
+
+@pytest.mark.parametrize("idx,far", [(torch.int32, 2 ** 31 - 1), (torch.int64, 2 ** 31), (torch.int64, 2 ** 40 + 12345),
+                                     (torch.int64, 2 ** 53 - 1)])
+def test_positions_far_out(cuda_device, idx, far):
+    """Angles from whole numbers and fractions: position x frequency (each exact) x 1 / 2 pi to 60 digits, whole turns dropped."""
+    turn = Fraction("0.159154943091895335768883763372514362034459645740456448747667")
+    q, k, pos, inv = _inputs(cuda_device, 24, 2, 1, 32, 16, 1, torch.float32)
+    pos = torch.tensor([[(far - i * (far // 1000)) * (-1) ** i for i in range(24)]], dtype=idx, device=cuda_device)
+    inv[3:6] = torch.tensor([1.9999998, 1.0 / 3, 1000.123])
+    angles = []
+    for p in pos[0].tolist():
+        turns = [p * Fraction(f) * turn for f in inv.tolist()]
+        angles.append([2 * math.pi * float(t - round(t)) for t in turns])
+    angle = torch.tensor(angles, dtype=torch.float64, device=cuda_device)[:, None]
+    for out, x in zip(apply_multi_axis_rotary(q, k, pos, inv, [16]), (q, k)):
+        lo, hi = x.double().chunk(2, -1)
+        _close(out, x, torch.cat([lo * angle.cos() - hi * angle.sin(), hi * angle.cos() + lo * angle.sin()], -1), 16)
