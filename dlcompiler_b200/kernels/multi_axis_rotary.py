@@ -10,6 +10,7 @@ from typing import Sequence
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from .. import _lib
 
@@ -57,34 +58,50 @@ def _rotated(q, k, positions, inv_freq, axes, inverse, q_out=None, k_out=None):
     return q_out, k_out
 
 
+def _has_tangent(*tensors):
+    """Does one of them carry a tangent of forward-mode differentiation?"""
+    return forward_ad._current_level >= 0 and any(
+        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 class _MultiAxisRotary(torch.autograd.Function):
-    """The gradient of a rotation is the rotation back, so the backward pass is the same launch with the other sign (and, where
-    it is to be differentiated again, this function)."""
+    """A rotation is linear and its transpose the rotation back: tangents take the same launch, gradients the one with the
+    other sign (and, where they are to be differentiated again, this function)."""
 
     @staticmethod
     def forward(ctx, q, k, positions, inv_freq, axes, inverse):
         ctx.save_for_backward(positions, inv_freq)
-        ctx.axes, ctx.inverse = axes, inverse
+        ctx.save_for_forward(positions, inv_freq)
+        ctx.axes, ctx.inverse, ctx.shapes = axes, inverse, (q.shape, k.shape)
         ctx.set_materialize_grads(False)
         return _rotated(q, k, positions, inv_freq, axes, inverse)
 
     @staticmethod
+    def _rotate_some(ctx, q, k, inverse):
+        """One of the two may be None: its heads are left out of the launch."""
+        if q is None and k is None:
+            return None, None
+        positions, inv_freq = ctx.saved_tensors
+        some = k if q is None else q
+        none = some.new_empty((some.size(0), 0, some.size(2))) if q is None or k is None else None
+        rotate = _MultiAxisRotary.apply if torch.is_grad_enabled() or _has_tangent(q, k) else _rotated
+        q_out, k_out = rotate(none if q is None else q, none if k is None else k, positions, inv_freq, ctx.axes, inverse)
+        return None if q is None else q_out, None if k is None else k_out
+
+    @staticmethod
     def backward(ctx, grad_q, grad_k):
-        # an output that nothing was made of has no gradient, an input may want none: their heads are left out of the launch
+        # an output that nothing was made of has no gradient, an input may want none
         if not ctx.needs_input_grad[0]:
             grad_q = None
         if not ctx.needs_input_grad[1]:
             grad_k = None
-        if grad_q is None and grad_k is None:
-            return (None,) * 6
-        positions, inv_freq = ctx.saved_tensors
-        if grad_q is None or grad_k is None:
-            some = grad_k if grad_q is None else grad_q
-            none = some.new_empty((some.size(0), 0, some.size(2)))
-        rotate = _MultiAxisRotary.apply if torch.is_grad_enabled() else _rotated
-        dq, dk = rotate(none if grad_q is None else grad_q, none if grad_k is None else grad_k, positions, inv_freq,
-                        ctx.axes, not ctx.inverse)
-        return None if grad_q is None else dq, None if grad_k is None else dk, None, None, None, None
+        return *_MultiAxisRotary._rotate_some(ctx, grad_q, grad_k, not ctx.inverse), None, None, None, None
+
+    @staticmethod
+    def jvp(ctx, q_tangent, k_tangent, *_):
+        some = k_tangent if q_tangent is None else q_tangent
+        out = _MultiAxisRotary._rotate_some(ctx, q_tangent, k_tangent, ctx.inverse)
+        return tuple(some.new_zeros(shape) if t is None else t for t, shape in zip(out, ctx.shapes))    # none is not taken
 
 
 def apply_multi_axis_rotary(
@@ -107,8 +124,8 @@ def apply_multi_axis_rotary(
     one rounding to the tensors' type (fp16, bf16, fp32): no cos / sin tables, and angles as good far out, up to position
     2^53, as near 0.
 
-    Differentiable in q and k where one of them requires a gradient; `q_embed` / `k_embed` (which may be the inputs)
-    are for calls without one.  Returns (q_embed, k_embed).
+    Differentiable in q and k, backward and forward (`torch.autograd.forward_ad`), more than once; `q_embed` / `k_embed` (which may
+    be q and k themselves) are for calls without a gradient or tangent.  Returns (q_embed, k_embed).
     """
     dev = _lib.require_cuda(q, k, positions, inv_freq, q_embed, k_embed)
     assert q.dim() == 3 and k.dim() == 3 and positions.dim() == 2, "q and k are [tokens, heads, dim], positions [axes, tokens]"
@@ -117,12 +134,12 @@ def apply_multi_axis_rotary(
     assert k.dtype is q.dtype, "q and k must have one dtype"
     assert positions.dtype is torch.int64 or positions.dtype is torch.int32, "positions must be int32 or int64"
     assert inv_freq.dim() == 1 and inv_freq.dtype is torch.float32, "inv_freq is a vector of fp32"
-    assert not inv_freq.requires_grad, "there is no gradient for inv_freq"
+    assert not (inv_freq.requires_grad or _has_tangent(inv_freq)), "there is no gradient for inv_freq"
     axes = _axis_of_freq(tuple(sections), bool(interleaved), n_axes, inv_freq.numel())
     if positions.stride(1) != 1:
         positions = positions.contiguous()
     inv_freq = inv_freq.contiguous()
-    if (q.requires_grad or k.requires_grad) and torch.is_grad_enabled():
-        assert q_embed is None and k_embed is None, "outputs cannot be given where a gradient is wanted"
+    if (q.requires_grad or k.requires_grad) and torch.is_grad_enabled() or _has_tangent(q, k):
+        assert q_embed is None and k_embed is None, "outputs cannot be given where a gradient or tangent is wanted"
         return _MultiAxisRotary.apply(q, k, positions, inv_freq, axes, False)
     return _rotated(q, k, positions, inv_freq, axes, False, q_embed, k_embed)

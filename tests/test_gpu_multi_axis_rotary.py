@@ -4,6 +4,7 @@ from fractions import Fraction
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwAD
 
 from dlcompiler_b200 import apply_multi_axis_rotary, apply_rotary_pos_emb
 
@@ -207,3 +208,49 @@ def test_positions_far_out(cuda_device, idx, far):
     for out, x in zip(apply_multi_axis_rotary(q, k, pos, inv, [16]), (q, k)):
         lo, hi = x.double().chunk(2, -1)
         _close(out, x, torch.cat([lo * angle.cos() - hi * angle.sin(), hi * angle.cos() + lo * angle.sin()], -1), 16)
+
+
+@pytest.mark.parametrize("dtype,dim,half", [(torch.bfloat16, 64, 32), (torch.float32, 13, 4)])
+def test_forward_mode(cuda_device, dtype, dim, half):
+    """The map is linear: an output's tangent is the rotation of the input's, an input without one gives none."""
+    q, k, pos, inv = _inputs(cuda_device, 11, 4, 2, dim, half, 2, dtype)
+    sections, (tq, tk) = [half // 2, half - half // 2], (torch.randn_like(t) for t in (q, k))
+    plain, turned = (apply_multi_axis_rotary(a, b, pos, inv, sections) for a, b in ((q, k), (tq, tk)))
+    for wants in (False, True):
+        with fwAD.dual_level():
+            for with_q, with_k in ((True, True), (True, False), (False, True)):
+                a = fwAD.make_dual(q.clone().requires_grad_(wants), tq) if with_q else q
+                b = fwAD.make_dual(k.clone().requires_grad_(wants), tk) if with_k else k
+                for out, value, tangent, has in zip(apply_multi_axis_rotary(a, b, pos, inv, sections), plain, turned, (with_q, with_k)):
+                    out = fwAD.unpack_dual(out)
+                    assert torch.equal(out.primal, value)
+                    if has:
+                        assert torch.equal(out.tangent, tangent)
+                    else:
+                        assert out.tangent is None or not out.tangent.any()
+            with torch.no_grad():
+                out, _ = apply_multi_axis_rotary(fwAD.make_dual(q, tq), k, pos, inv, sections)
+                assert torch.equal(fwAD.unpack_dual(out).tangent, turned[0])
+
+
+def test_forward_mode_of_the_gradient(cuda_device):
+    """The gradient is linear in the incoming one: its tangent is turned back."""
+    q, k, pos, inv = _inputs(cuda_device, 11, 4, 2, 16, 8, 2, torch.float32)
+    q.requires_grad_()
+    g, tg = torch.randn_like(q), torch.randn_like(q)
+    back, = torch.autograd.grad(apply_multi_axis_rotary(q, k, pos, inv, [4, 4])[0], q, tg)
+    for create in (False, True):
+        with fwAD.dual_level():
+            out, _ = apply_multi_axis_rotary(q, k, pos, inv, [4, 4])
+            dq, = torch.autograd.grad(out, q, fwAD.make_dual(g, tg), create_graph=create)
+            assert torch.equal(fwAD.unpack_dual(dq).tangent, back)
+
+
+def test_forward_mode_refusals(cuda_device):
+    """A tangent that would be lost: into given outputs, and of the frequencies."""
+    q, k, pos, inv = _inputs(cuda_device, 3, 2, 1, 16, 8, 1, torch.float32)
+    with fwAD.dual_level():
+        with pytest.raises(AssertionError, match="outputs"):
+            apply_multi_axis_rotary(fwAD.make_dual(q, q), k, pos, inv, [8], q_embed=torch.empty_like(q))
+        with pytest.raises(AssertionError, match="inv_freq"):
+            apply_multi_axis_rotary(q, k, pos, fwAD.make_dual(inv, inv), [8])
