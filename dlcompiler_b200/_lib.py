@@ -25,6 +25,7 @@ _DTYPES = {torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16, torch.float32: 
 SIGNATURES = {
     "dlb_version": (c_int, []),
     "dlb_last_error": (c_char_p, []),
+    "dlb_status_word": (c_int, [c_void_p]),
     "dlb_set_wait_budget_ms": (c_int, [c_int64]),
     "dlb_moe_start_end": (c_int, [c_void_p, c_int, c_int64, c_int, c_void_p, c_void_p, c_int, c_void_p]),
     "dlb_silu_and_mul": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int, c_void_p]),
@@ -193,19 +194,33 @@ def require_cuda(*tensors: torch.Tensor) -> torch.device:
 _status_words: dict[int, torch.Tensor] = {}
 
 
+class _StatusMemory:
+    """A device's status word, which lies inside the library, for torch to look at."""
+
+    def __init__(self, address: int):
+        self.__cuda_array_interface__ = {"shape": (4,), "typestr": "<i4", "data": (address, False), "version": 3}
+
+
 def status_word(device: torch.device) -> torch.Tensor:
-    """Per-device int32[4] that a kernel writes when a bounded wait gives up or a table row or page does not exist."""
+    """Per-device int32[4] that a kernel writes when a bounded wait gives up or a table row or page does not exist.  It is
+    zero from the library's load on: a tensor filled on first use would be filled again by every replay where that use was
+    captured, and on a stream of one thread while another's kernels already write it."""
     idx = device.index if device.index is not None else torch.cuda.current_device()
     t = _status_words.get(idx)
     if t is None:
-        t = torch.zeros(4, dtype=torch.int32, device=device)
-        _status_words[idx] = t
+        device = torch.device("cuda", idx)
+        address = ctypes.c_void_p()
+        with on_device(device):
+            check(load().dlb_status_word(ctypes.byref(address)), "status_word")
+            t = torch.as_tensor(_StatusMemory(address.value), device=device)
+        assert t.data_ptr() == address.value, "status_word: torch copied the library's memory"
+        t = _status_words.setdefault(idx, t)
     return t
 
 
 def existing_status_word(device: torch.device):
-    """The device's status word if some earlier call created it, else None (the kernels take NULL).
-    For call paths that must not allocate."""
+    """The device's status word if some earlier call asked for it, else None (the kernels take NULL).
+    For call paths that must not create a tensor."""
     idx = device.index if device.index is not None else torch.cuda.current_device()
     return _status_words.get(idx)
 

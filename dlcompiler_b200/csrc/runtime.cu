@@ -12,6 +12,10 @@
 
 namespace dlb {
 
+// The word of every device that callers without one of their own hand to the kernels: zero from the library's load on, so that
+// no launch that writes it has to be ordered behind a launch that clears it.
+static __device__ int32_t g_status_word[4];
+
 static thread_local char g_last_error[512] = {0};
 
 void set_last_error(const char* fmt, ...) {
@@ -116,6 +120,16 @@ extern "C" {
 int dlb_version(void) { return 100; }
 
 const char* dlb_last_error(void) { return dlb::g_last_error; }
+
+int dlb_status_word(void** word) {
+  DLB_CHECK_ARG(word != nullptr, DLB_ERR_BAD_ARG, "status_word: null pointer");
+  const cudaError_t e = cudaGetSymbolAddress(word, dlb::g_status_word);
+  if (e != cudaSuccess) {
+    dlb::set_last_error("status_word: %s", cudaGetErrorString(e));
+    (void)cudaGetLastError();
+  }
+  return (int)e;
+}
 
 int dlb_set_wait_budget_ms(int64_t ms) {
   DLB_CHECK_ARG(ms >= 1 && ms <= 60000, DLB_ERR_BAD_ARG, "wait budget %lld ms not in [1, 60000]", (long long)ms);

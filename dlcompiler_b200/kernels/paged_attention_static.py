@@ -42,7 +42,7 @@ def paged_decode_no_alloc(q: Tensor, k: Tensor, v: Tensor, o: Tensor, block_offs
         chunk *= 2
         max_splits = (max_ctx + chunk - 1) // chunk
     lib = _lib.load()
-    # the status word is a torch tensor: use it only if an earlier call already made it (NULL is allowed)
+    # the status word comes as a torch tensor: use it only if an earlier call already made that (NULL is allowed)
     status = _lib.existing_status_word(dev)
     with _lib.on_device(dev):
         rc = lib.dlb_paged_decode_static(

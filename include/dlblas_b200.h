@@ -45,6 +45,9 @@ const char* dlb_last_error(void);
  * raises (expert-parallel kernels).  A wait that runs out writes `status` and the kernel goes on; it
  * never hangs.  Process-wide; applies to launches made after the call. */
 int dlb_set_wait_budget_ms(int64_t ms);
+/* Address of the current device's status word (int32[4] inside the library, zero at its load), to pass as `status`.  May be asked
+ * for while a stream is captured. */
+int dlb_status_word(void** word);
 
 /* silu_and_mul: out[t, i] = silu(x[t, i]) * x[t, n + i], fp32 math, one rounding.
  * Replaces python/dlBLAS/dlblas/kernels/activation.py:88-130 (wrapper) and :17-85 (kernels). */
