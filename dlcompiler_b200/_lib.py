@@ -237,9 +237,11 @@ def check_device_status(device=None) -> None:
         t = _status_words.get(idx)
         if t is None:
             continue
+        torch.cuda.synchronize(idx)              # every stream: the copy would wait for the current one alone
         vals = t.cpu().tolist()
         if vals[0] != 0:
             t.zero_()
+            torch.cuda.synchronize(idx)          # and later launches on other streams would not wait for the fill
             if vals[0] == DEV_BAD_ROW:
                 raise DlblasError(f"device status on cuda:{idx}: request {vals[1]} of a decode asked for row {vals[3]} "
                                   f"of a table of {vals[2]}")

@@ -79,3 +79,19 @@ threads = [threading.Thread(target=first) for _ in range(2)]
 assert len(words) == 2 and words[0].data_ptr() == words[1].data_ptr() == _lib.status_word(dev).data_ptr()
 assert words[0].tolist() == [0] * 4
 """)
+
+
+def test_check_waits_for_other_streams(cuda_device):
+    """A bad page behind a tenth of a second of other work on a stream that is not the current one."""
+    _fresh("""
+table[0, 1] = 9
+sinks()
+assert reported()
+side = torch.cuda.Stream()
+side.wait_stream(torch.cuda.current_stream())
+with torch.cuda.stream(side):
+    torch.cuda._sleep(200_000_000)
+    sinks()
+assert reported()
+table[0, 1] = 1
+""")
