@@ -254,3 +254,28 @@ def test_forward_mode_refusals(cuda_device):
             apply_multi_axis_rotary(fwAD.make_dual(q, q), k, pos, inv, [8], q_embed=torch.empty_like(q))
         with pytest.raises(AssertionError, match="inv_freq"):
             apply_multi_axis_rotary(q, k, pos, fwAD.make_dual(inv, inv), [8])
+
+
+def test_training_step_in_a_graph(cuda_device):
+    """Forward and backward captured together and replayed with other inputs, positions and incoming gradients."""
+    q, k, pos, inv = _inputs(cuda_device, 40, 4, 2, 64, 32, 3, torch.bfloat16)
+    q.requires_grad_(), k.requires_grad_()
+    gq, gk = (torch.randn_like(t) for t in (q, k))
+
+    def step():
+        qe, ke = apply_multi_axis_rotary(q, k, pos, inv, [16, 8, 8])
+        return (qe, ke) + torch.autograd.grad((qe, ke), (q, k), (gq, gk))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    with torch.no_grad():
+        pos += 17
+        q.mul_(-2), gk.mul_(3)
+    graph.replay()
+    assert all(torch.equal(a, b) for a, b in zip(outs, step()))

@@ -1,5 +1,9 @@
 """GPU: the serving operators together, as a server calls them: rotary positions of several axes for q and k, the keys and
 values into the paged cache, attention over it, with a window and sinks or behind a shared prefix."""
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 
@@ -180,3 +184,46 @@ def test_calls_from_several_threads(cuda_device, streams):
         t.join()
     assert not wrong
     check_device_status()
+
+
+def test_every_thread_gets_through(cuda_device):
+    """Threads on streams of their own from a process's first call on; an exception in one of them is a failure."""
+    code = """
+import threading
+from concurrent.futures import ThreadPoolExecutor
+import torch
+from dlcompiler_b200 import apply_multi_axis_rotary, check_device_status, shared_prefix_attention_fwd, sink_attention_fwd
+dev, n = torch.device("cuda:0"), 4
+g = torch.Generator().manual_seed(5)
+k, v = (torch.randn(30, 16, 2, 64, generator=g).to(torch.bfloat16).to(dev) for _ in range(2))
+q = torch.randn(6, 8, 64, generator=g).to(torch.bfloat16).to(dev)
+table = torch.randperm(30, generator=g).view(6, 5).int().to(dev)
+lens, start, one = (torch.tensor(x, dtype=torch.int32, device=dev) for x in ([5, 17, 33, 48, 70, 79], list(range(6)), [1] * 6))
+groups, inv = torch.tensor([0, 2, 6], dtype=torch.int32, device=dev), torch.ones(32, device=dev)
+torch.cuda.synchronize()
+gate = threading.Barrier(n)
+
+def step():
+    a, _ = apply_multi_axis_rotary(q, q[:, :2], lens.long()[None], inv, [32])
+    b = sink_attention_fwd(a, k, v, torch.empty_like(a), table, start, one, lens, 1, 31, 4)
+    c = sink_attention_fwd(a, k, v, torch.empty_like(a), table, start, one, lens, 2, 31, 4)
+    return a, b, c, shared_prefix_attention_fwd(a, k, v, torch.empty_like(a), table[:2], lens[4:], groups, table, lens)
+
+def work(i):
+    gate.wait()
+    with torch.cuda.stream(torch.cuda.Stream()):
+        outs = [step() for _ in range(50)]
+    torch.cuda.synchronize()
+    return outs
+
+with ThreadPoolExecutor(n) as pool:
+    done = [f.result() for f in [pool.submit(work, i) for i in range(n)]]
+ref = step()
+assert len(done) == n and all(len(outs) == 50 for outs in done)
+assert all(torch.equal(x, y) for outs in done for got in outs for x, y in zip(got, ref))
+check_device_status()
+print("all through")
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    res = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=600)
+    assert res.returncode == 0 and "all through" in res.stdout, res.stdout + res.stderr
