@@ -71,7 +71,8 @@ class _MultiAxisRotary(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, positions, inv_freq, axes, inverse):
         ctx.save_for_backward(positions, inv_freq)
-        ctx.save_for_forward(positions, inv_freq)
+        if forward_ad._current_level >= 0:
+            ctx.save_for_forward(positions, inv_freq)
         ctx.axes, ctx.inverse, ctx.shapes = axes, inverse, (q.shape, k.shape)
         ctx.set_materialize_grads(False)
         return _rotated(q, k, positions, inv_freq, axes, inverse)
