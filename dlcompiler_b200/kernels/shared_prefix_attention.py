@@ -69,7 +69,10 @@ def shared_prefix_attention_fwd(
     prefix, lengths may be zero, and a query without any key gets zeros.
 
     The prefix is cut into splits that all sequences of a group go through together as the rows of matrix products; the
-    partial results wait in a workspace and join the sequences' own tokens in the second of two launches.  A page
+    partial results wait in a workspace and join the sequences' own tokens in the second of two launches.  Lengths stay on the
+    device, so splits, workspace and the CTAs for the own tokens (at most 8 to a sequence and key head) are planned from the widths
+    of the two tables: pass them about as wide as the longest entry needs (8 sequences behind 4000 tokens: 20 us, with a prefix
+    table of 131072 tokens 27).  A page
     outside the cache where a token should be is an error (`check_device_status()` raises).  Types, head sizes, pages
     and alignment as in `sink_attention_fwd`.
     """

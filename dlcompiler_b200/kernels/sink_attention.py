@@ -80,6 +80,11 @@ def sink_attention_fwd(
     query that sees no key gets zeros.  Where `kv_seqlens` is past what a row of `block_offsets` has room for, queries keep their
     positions and the tokens past the table are not there.
 
+    The form for single tokens is one launch without a workspace, in which at most 8 CTAs share the keys of a sequence and key
+    head: made for windows of some thousand keys, or batches that fill the GPU.  A few sequences behind a window of 100000 keys
+    and more are better served by `paged_attention_fwd` where there are no sinks to keep (one sequence, one key head, 131072 keys:
+    178 us here, 123 there).
+
     Only pages with a token that some query of a tile of 128 rows sees are looked at: entries of `block_offsets` for
     tokens behind the window may be stale.  A page outside the cache where a visible token should be is an error
     (`check_device_status()` raises), and its sequence's output is undefined.  fp16/bf16, head sizes multiples of 8 up
