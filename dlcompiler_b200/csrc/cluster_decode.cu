@@ -72,6 +72,7 @@ cluster_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
   uint64_t* empty_bar = full_bar + STAGES;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(empty_bar + STAGES);
   volatile int* ext_splits = abort_flag + 1;
+  volatile int* loaded = abort_flag + 2;                     // tiles that were asked for
 
   const int rank = blockIdx.x, cluster = gridDim.x;
   const int kvh = blockIdx.y % p.hkv;
@@ -159,7 +160,7 @@ cluster_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
       const int64_t column = lane_token(t, wanted) >> p.page_shift;
       return wanted ? clamped_index(p.block_table, (int64_t)b * p.bt_stride + column, p.table_is_int64) : 0;
     };
-    int pages = 0, pages_next = entry(t_lo);
+    int pages = 0, pages_next = entry(t_lo), asked = 0;
     for (int t = t_lo; t < t_hi; ++t) {
       const int i = t - t_lo, in_batch = i % batch_tiles;
       if (in_batch == 0) {
@@ -188,6 +189,7 @@ cluster_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
       }
       ok = __shfl_sync(0xffffffffu, ok, 0);
       if (!ok) break;
+      asked = i + 1;
       const int page = __shfl_sync(0xffffffffu, pages, in_batch * units + (min(lane << box_shift, TILE - 1) >> unit_shift));
       if (mine) {
         uint8_t* kdst = smem + s * L::STAGE_BYTES + (lane << box_shift) * 128;
@@ -201,6 +203,7 @@ cluster_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
         }
       }
     }
+    if (lane == 0) *loaded = asked;
   } else {
     // ------------------------------ consumers ------------------------------
     // Q^T as the B operand: head lane / 4 (of each block of 8), columns (lane & 3) * 2 of every 8
@@ -366,6 +369,10 @@ cluster_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
 
   // ------------------------------ join the warps ------------------------------
   __syncthreads();   // every load has been consumed: the ring can be reused
+  if (*abort_flag) {
+    if (threadIdx.x == 0) settle_ring(full_bar, STAGES, *loaded);
+    __syncthreads();
+  }
   constexpr int H = L::HEADS, PITCH = L::PITCH, QUADS = D / 4;
   float* red_o = reinterpret_cast<float*>(smem);             // [warps + 1][H][PITCH], the last one the CTA's
   float* red_m = red_o + (CONSUMERS + 1) * H * PITCH;        // [warps + 1][H]

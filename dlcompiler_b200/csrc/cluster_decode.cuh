@@ -120,6 +120,17 @@ __device__ __forceinline__ void soft_cap_any(float& a, float& b, const SoftCapSh
   b = fabsf(b * x) <= 0.25f ? lb : soft_cap(b, in, out);
 }
 
+// Behind a wait that gave up: waits, again with a limit, for what is still under way to a ring of barriers (copies, commits of
+// matrix instructions), so that nothing lands in the shared memory of a CTA that has left.  `used` uses of the ring have begun.
+__device__ __forceinline__ void settle_ring(uint64_t* ring, int stages, int used) {
+  for (int s = 0; s < stages && s < used; ++s) {
+    const uint32_t last = (uint32_t)((used - 1 - s) / stages) & 1;
+    const uint64_t t0 = globaltimer_ns();
+    while (!mbar_try_wait(&ring[s], last) && globaltimer_ns() - t0 < DLB_WAIT_BUDGET_NS) {
+    }
+  }
+}
+
 __device__ __forceinline__ void cluster_barrier() {
   asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }

@@ -235,6 +235,7 @@ packed_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
   uint64_t* p_full = pv_done + STAGES;       // [S_BUFS] P written
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(p_full + S_BUFS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile int* begun = abort_flag + 1;      // [4] blocks whose K and V loads, Q K^T and P V have begun
 
   if (warp == WARP_TMA && lane == 0) {
     mbar_init(q_full, 1);
@@ -246,6 +247,7 @@ packed_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
     }
     for (int h = 0; h < S_BUFS; ++h) mbar_init(&p_full[h], 128);
     *abort_flag = 0;
+    begun[0] = begun[1] = begun[2] = begun[3] = 0;
     fence_mbar_init();
   }
   if (warp == WARP_MMA) {
@@ -292,7 +294,7 @@ packed_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
         return wanted(j) ? clamped_index(p.block_table, (int64_t)seq * p.bt_stride + (lane_key(j) >> p.page_shift), p.table_is_int64)
                          : 0;
       };
-      int pages = 0, pages_next = entry(0);
+      int pages = 0, pages_next = entry(0), k_begun = 0, v_begun = 0;
       for (int j = 0; j < nb; ++j) {
         const int in_batch = j & (batch - 1);
         if (in_batch == 0) {
@@ -326,6 +328,7 @@ packed_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
         }
         ok = __shfl_sync(0xffffffffu, ok, 0);
         if (!ok) break;
+        k_begun = j + 1;
         if (fetch) load(dst + OFF_K, &tmap_k, &k_full[s], p.k_whole);
         if (lane == 0) {
           ok = mbar_wait(&pv_done[s], ph ^ 1, abort_flag, p.status, 52, j) ? 1 : 0;
@@ -333,7 +336,12 @@ packed_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
         }
         ok = __shfl_sync(0xffffffffu, ok, 0);
         if (!ok) break;
+        v_begun = j + 1;
         if (fetch) load(dst + OFF_V, &tmap_v, &v_full[s], p.v_whole);
+      }
+      if (lane == 0) {
+        begun[0] = k_begun;
+        begun[1] = v_begun;
       }
     }
   } else if (warp == WARP_MMA) {
@@ -348,6 +356,7 @@ packed_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
       const uint32_t q_lo0 = (uint32_t)q_d0, k_lo0 = (uint32_t)k_d0, kq_hi = (uint32_t)(q_d0 >> 32);
       const uint32_t v_lo0 = (uint32_t)v_d0, v_hi = (uint32_t)(v_d0 >> 32);
       constexpr int AHEAD = S_BUFS - 1;                        // P V comes that many blocks after Q K^T
+      int qk_begun = 0, pv_begun = 0;
       for (int j = 0; ok && j < nb + AHEAD; ++j) {
         if (j < nb) {
           // S_j = Q K_j^T
@@ -363,6 +372,7 @@ packed_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
             else umma_ss_lohi<1>(tmem_base + (j % S_BUFS) * BN, q_lo0 + qoff, kq_hi, k_lo + koff, kq_hi, p.idesc_qk);
           }
           umma_commit(&qk_done[s]);
+          qk_begun = j + 1;
         }
         if (j >= AHEAD) {
           // O += P V of block jj
@@ -380,8 +390,11 @@ packed_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
 #pragma unroll
           for (int ks = 1; ks < BN / 16; ++ks) umma_ts_lohi<1>(tmem_o, pt + ks * 8, v_lo + ks * (16 * 128 >> 4), v_hi, p.idesc_pv);
           umma_commit(&pv_done[s]);
+          pv_begun = jj + 1;
         }
       }
+      begun[2] = qk_begun;
+      begun[3] = pv_begun;
     }
   } else {
     // ------------------------------ softmax / correction ------------------------------
@@ -651,6 +664,16 @@ packed_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
 
   tc_fence_before_sync();
   __syncthreads();
+  if (*abort_flag) {
+    if (threadIdx.x == 0) {
+      if (nb > 0) settle_ring(q_full, 1, 1);
+      settle_ring(k_full, STAGES, begun[0]);
+      settle_ring(v_full, STAGES, begun[1]);
+      settle_ring(qk_done, STAGES, begun[2]);
+      settle_ring(pv_done, STAGES, begun[3]);
+    }
+    __syncthreads();
+  }
   if (warp == WARP_MMA) {
     tc_fence_after_sync();
     tmem_dealloc(tmem_base, TMEM_COLS);
