@@ -135,12 +135,13 @@ def apply_multi_axis_rotary(
     assert k.dtype is q.dtype, "q and k must have one dtype"
     assert positions.dtype is torch.int64 or positions.dtype is torch.int32, "positions must be int32 or int64"
     assert inv_freq.dim() == 1 and inv_freq.dtype is torch.float32, "inv_freq is a vector of fp32"
-    assert not (inv_freq.requires_grad or _has_tangent(inv_freq)), "there is no gradient for inv_freq"
+    dual = forward_ad._current_level >= 0              # tangents are looked for only where there may be some
+    assert not (inv_freq.requires_grad or dual and _has_tangent(inv_freq)), "there is no gradient for inv_freq"
     axes = _axis_of_freq(tuple(sections), bool(interleaved), n_axes, inv_freq.numel())
     if positions.stride(1) != 1:
         positions = positions.contiguous()
     inv_freq = inv_freq.contiguous()
-    if (q.requires_grad or k.requires_grad) and torch.is_grad_enabled() or _has_tangent(q, k):
+    if (q.requires_grad or k.requires_grad) and torch.is_grad_enabled() or dual and _has_tangent(q, k):
         assert q_embed is None and k_embed is None, "outputs cannot be given where a gradient or tangent is wanted"
         return _MultiAxisRotary.apply(q, k, positions, inv_freq, axes, False)
     return _rotated(q, k, positions, inv_freq, axes, False, q_embed, k_embed)
